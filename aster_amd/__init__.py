@@ -9,6 +9,7 @@ PagedAttentionRunner) and a C-ABI library of hand-written HIP kernels
 """
 
 from .attention_backend import BACKEND, AttentionWork, KernelWork, UnsupportedAttentionBackend
+from .key_weights import EvictedTokens, KeyWeightRows, KeyWeights
 from .kv_quantization import KVQuantization, QuantizedKV, quantize_kv
 from .offload import PagedStateArchive
 from .online_attention import (AttentionBlock, SoftmaxState, merge_softmax, online_attention,
@@ -25,5 +26,6 @@ __all__ = [
     "KVStateCodec", "PagedStatePool", "PagedSequence", "PageRef", "PageView", "SlotReservation",
     "StateError", "CacheCapacityError", "PagedStateArchive", "PagedAttentionRunner",
     "PagedAttentionStep", "PrefixPacks", "plan_prefix_packs", "AttentionBlock", "SoftmaxState",
-    "merge_softmax", "online_attention", "online_attention_statistics",
+    "merge_softmax", "online_attention", "online_attention_statistics", "KeyWeights",
+    "KeyWeightRows", "EvictedTokens",
 ]

@@ -46,6 +46,10 @@ EXPORTED_SYMBOLS = (
     "astr_paged_attention_i8_planned_workspace_bytes",
     "astr_paged_attention_i8_planned",
     "astr_paged_attention_i8_planned_append",
+    "astr_paged_attention_i8_sinks",
+    "astr_paged_attention_i8_key_weights",
+    "astr_paged_attention_i8_bounded_workspace_bytes",
+    "astr_kv_evict",
     "astr_last_error",
     "astr_version",
 )
@@ -69,6 +73,19 @@ class PagedKVDesc(ctypes.Structure):
         ("head_dim", ctypes.c_int32),
         ("key_valid", ctypes.c_void_p),
         ("code_format", ctypes.c_int32),
+    ]
+
+
+class KeyWeightsDesc(ctypes.Structure):
+    """Mirror of ``astr_key_weights``."""
+
+    _fields_ = [
+        ("values", ctypes.c_void_p),
+        ("row_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+        ("rows", ctypes.c_void_p),
+        ("num_rows", ctypes.c_int32),
+        ("capacity", ctypes.c_int32),
     ]
 
 
@@ -160,6 +177,22 @@ def lib():
             c_i64, c_i64, c_vp, c_vp, c_i32, ctypes.c_float, c_vp, c_vp, c_vp, c_sz, c_vp, c_vp,
         ]
         handle.astr_paged_attention_i8_planned_append.restype = ctypes.c_int
+        weights_p = ctypes.POINTER(KeyWeightsDesc)
+        bounded = [desc_p, c_vp, c_i32, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_i32, c_i32,
+                   c_vp, c_i32, c_vp, c_i32, c_i32, c_i32, ctypes.c_float]
+        handle.astr_paged_attention_i8_sinks.argtypes = bounded + [c_i32, c_i32, c_vp, c_sz, c_vp,
+                                                                   c_vp]
+        handle.astr_paged_attention_i8_sinks.restype = ctypes.c_int
+        handle.astr_paged_attention_i8_key_weights.argtypes = bounded + [weights_p, c_vp, c_sz,
+                                                                         c_vp, c_vp]
+        handle.astr_paged_attention_i8_key_weights.restype = ctypes.c_int
+        handle.astr_paged_attention_i8_bounded_workspace_bytes.argtypes = [c_i32] * 11
+        handle.astr_paged_attention_i8_bounded_workspace_bytes.restype = c_sz
+        handle.astr_kv_evict.argtypes = [
+            desc_p, c_i32, c_i64, c_i64, weights_p, c_i64, c_vp, c_vp, c_i32, c_vp, c_i32, c_vp,
+            c_i32, c_i32, c_i32, c_i32, c_i32, c_vp, c_vp, c_vp, c_vp,
+        ]
+        handle.astr_kv_evict.restype = ctypes.c_int
         handle.astr_last_error.argtypes = []
         handle.astr_last_error.restype = ctypes.c_char_p
         handle.astr_version.argtypes = []

@@ -21,10 +21,12 @@ OUT_DIR = os.path.join(HERE, "_lib")
 OUT = os.path.join(OUT_DIR, "libaster_kv.so")
 SOURCES = ("errors.hip", "kv_quantize.hip", "paged_attention.hip", "decode_partition.hip",
            "decode_streamk.hip", "decode_planned.hip", "prefill.hip", "kv_copy.hip",
-           "softmax_merge.hip", "decode_plan.cpp")
+           "softmax_merge.hip", "decode_plan.cpp", "bounded_attention.hip", "decode_bounded.hip",
+           "chunk_weights.hip", "kv_evict.hip")
 # attention kernels built once per KV code format (int8, FP8 E4M3FN, FP8 E5M2):
 # -DASTR_KF=k selects the format of that object's instantiations
-PER_FORMAT = ("decode_partition.hip", "decode_streamk.hip", "decode_planned.hip", "prefill.hip")
+PER_FORMAT = ("decode_partition.hip", "decode_streamk.hip", "decode_planned.hip", "prefill.hip",
+              "decode_bounded.hip", "chunk_weights.hip")
 FORMATS = (0, 1, 2)
 
 
@@ -49,6 +51,9 @@ def units(trace=False):
                             [f"-DASTR_KF={k}", "-DASTR_SK_PART=2", *STREAMK_PLAIN_FLAGS]))
         elif s in PER_FORMAT:
             out += [(s, f"{stem}_kf{k}", [f"-DASTR_KF={k}"]) for k in FORMATS]
+            if s == "prefill.hip":  # once more for windows with sinks
+                out += [(s, f"{stem}_sinks_kf{k}", [f"-DASTR_KF={k}", "-DASTR_PF_SINKS=1"])
+                        for k in FORMATS]
         else:
             out.append((s, stem, []))
     return out

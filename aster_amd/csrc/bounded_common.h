@@ -1,0 +1,115 @@
+// Arguments and launchers of the operators that keep a paged cache bounded (gfx950):
+// attention in which the first tokens stay visible beside a sliding window, and attention
+// that adds up each key's softmax weight.
+#pragma once
+
+#include "attention_common.h"
+
+namespace astr {
+namespace attn {
+
+// The weights gathered per key: row `rows[s]` (s without `rows`) of sequence s, KV head h,
+// key t at values[row * row_stride + h * head_stride + t], t < capacity.
+struct KeyWeights {
+  float* values;
+  int64_t row_stride, head_stride;
+  const int32_t* rows;
+  int32_t num_rows, capacity;
+};
+
+struct BoundedArgs : AttnArgs {
+  int32_t sinks;        // keys [0, sinks) stay visible beside the window
+  int32_t max_context;  // host bound of context_lens
+  int32_t group;        // query heads per KV head
+  // decode: a row's visible blocks in pieces of part_blocks (AttnArgs), at most max_parts
+  KeyWeights kw;
+  // base-2 scores of every key, [num_seqs * num_kv_heads * group][score_stride]; weights only
+  float* scores;
+  int64_t score_stride;
+  // chunks (key weights): (m, l) of every (query token, head) and piece of its keys,
+  // [piece][num_q_tokens][num_q_heads], and the pieces' key steps of 64
+  float* chunk_ml;
+  int32_t chunk_pieces, chunk_steps;
+};
+
+// What sequence `seq` sees: keys [0, sinks) in blocks [0, sink_blocks) and keys [kv_begin,
+// ctx) in blocks [first_blk, last_blk), as one list of blocks. No sink block of its own
+// where the window reaches the sinks. A block that holds keys of both is listed twice, each
+// time with the bounds of one.
+struct VisibleList {
+  int ctx, kv_begin, sink_end, sink_blocks, first_blk, blocks;
+  __device__ __forceinline__ int block(int f) const {
+    return f < sink_blocks ? f : first_blk + f - sink_blocks;
+  }
+  __device__ __forceinline__ int lo(int f) const { return f < sink_blocks ? 0 : kv_begin; }
+  __device__ __forceinline__ int hi(int f) const { return f < sink_blocks ? sink_end : ctx; }
+};
+
+// A length outside the table or past the host's bound is reported and cut.
+__device__ __forceinline__ int bounded_ctx(const BoundedArgs& a, int ctx, bool report) {
+  const int64_t table = (int64_t)a.bt_stride * kBlockTokens;
+  const int cap = (int)(table < a.max_context ? table : a.max_context);
+  if (ctx < 0 || ctx > cap) {
+    if (report) atomicOr(a.err_flag, ASTR_FLAG_BAD_INDEX);
+    ctx = ctx < 0 ? 0 : cap;
+  }
+  return ctx;
+}
+
+__device__ __forceinline__ VisibleList visible_list(const BoundedArgs& a, int ctx) {
+  VisibleList v;
+  v.ctx = ctx;
+  const int begin = a.window > 0 && ctx > a.window ? ctx - a.window : 0;
+  const bool apart = a.sinks < begin;
+  v.kv_begin = apart ? begin : 0;
+  v.sink_end = apart ? a.sinks : 0;
+  v.sink_blocks = (v.sink_end + kBlockTokens - 1) / kBlockTokens;
+  v.first_blk = v.kv_begin / kBlockTokens;
+  v.blocks = v.sink_blocks + (ctx + kBlockTokens - 1) / kBlockTokens - v.first_blk;
+  return v;
+}
+
+// The weights' row of sequence `seq`, or -1 (reported) where its number is out of range.
+__device__ __forceinline__ int64_t weight_row(const BoundedArgs& a, int seq, bool report) {
+  const int row = a.kw.rows != nullptr ? a.kw.rows[seq] : seq;
+  if ((unsigned)row >= (unsigned)a.kw.num_rows) {
+    if (report) atomicOr(a.err_flag, ASTR_FLAG_BAD_INDEX);
+    return -1;
+  }
+  return row;
+}
+
+template <int KF> int launch_bounded_kf(const BoundedArgs& a, int32_t q_dtype, hipStream_t stream);
+template <int KF> int launch_chunk_weights_kf(const BoundedArgs& a, int32_t q_dtype, hipStream_t stream);
+// the chunked-prefill kernels with sinks (prefill.hip)
+struct SinkChunkArgs : ChunkArgs {
+  int32_t sinks;
+};
+template <int KF> int launch_prefill_sinks_kf(const SinkChunkArgs& a, int32_t q_dtype, hipStream_t stream);
+#define ASTR_DECLARE_BOUNDED(KF)                                                             \
+  template <> int launch_bounded_kf<KF>(const BoundedArgs&, int32_t, hipStream_t);           \
+  template <> int launch_chunk_weights_kf<KF>(const BoundedArgs&, int32_t, hipStream_t);     \
+  template <> int launch_prefill_sinks_kf<KF>(const SinkChunkArgs&, int32_t, hipStream_t);
+ASTR_DECLARE_BOUNDED(kInt8)
+ASTR_DECLARE_BOUNDED(kE4M3)
+ASTR_DECLARE_BOUNDED(kE5M2)
+#undef ASTR_DECLARE_BOUNDED
+
+#define ASTR_BY_FORMAT(name, Args)                                               \
+  inline int name(const Args& a, int32_t q_dtype, hipStream_t stream) {          \
+    switch (a.cache.code_format) {                                               \
+      case kInt8: return name##_kf<kInt8>(a, q_dtype, stream);                   \
+      case kE4M3: return name##_kf<kE4M3>(a, q_dtype, stream);                   \
+      default: return name##_kf<kE5M2>(a, q_dtype, stream);                     \
+    }                                                                            \
+  }
+ASTR_BY_FORMAT(launch_bounded, BoundedArgs)
+ASTR_BY_FORMAT(launch_chunk_weights, BoundedArgs)
+ASTR_BY_FORMAT(launch_prefill_sinks, SinkChunkArgs)
+#undef ASTR_BY_FORMAT
+
+// Waves of the decode kernel's workgroup: four, or as many as the LDS holds stages for.
+constexpr int wide_waves(int head_dim) { return head_dim == 256 ? 8 : 16; }
+
+}  // namespace attn
+}  // namespace astr

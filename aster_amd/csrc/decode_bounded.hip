@@ -1,0 +1,516 @@
+// Paged decode attention of a bounded cache (gfx950): rows of one query token at position
+// p = ctx - 1, which see
+//   keys k > p - window, and k < sinks  (window > 0), or every key;
+// with WEIGHTS each key's softmax weight, summed over the heads of its group, is added to
+// the weights kept per key and KV head:
+//   A[k] += sum_g exp(s_gk - lse_g),  lse_g = log sum_k exp(s_gk).
+//
+// One workgroup of NW waves takes a (sequence, KV head), or one of the equal pieces of its
+// visible blocks; wave w the blocks w, w + NW, ... of them, each 16-token block staged in
+// LDS by direct global -> LDS loads, two ahead, and through the MFMAs for all heads of the
+// group at once, so that each K/V byte is read from HBM once. The waves' states merge in
+// LDS, the pieces' in a second launch (one row's blocks alone cannot fill the GPU).
+// The scores do not stay on the chip: with WEIGHTS they are stored as they are formed (4
+// bytes a key and head, against 2 D + 8 of its codes and scales) and read again, from the
+// cache, once lse is known; reading the keys again instead would double the call's bytes.
+//
+// Queries of 16 bits: int8 codes meet three int8 terms of the query (exact products, 22
+// bits of the query), FP8 codes an f16 query; softmax weights enter the output's products
+// rounded to f16, the sums in fp32 before that rounding. fp32 queries: FP8 codes meet two
+// f16 terms of the query, and the weights enter as two f16 terms (22 bits).
+#include <type_traits>
+
+#include "bounded_common.h"
+
+namespace astr {
+namespace attn {
+namespace {
+
+#ifndef ASTR_KF
+#define ASTR_KF 0
+#endif
+constexpr int KF = ASTR_KF;  // this translation unit's code format
+
+constexpr int kTileTokens = 1024;  // keys whose weights one workgroup of the second launch adds
+
+// The FP8 query operand: f16 terms of the query column, scaled by the power of two that
+// brings its largest element into [2^14, 2^15) (then exact for 16-bit queries, whose
+// elements below 2^-28 of that maximum round by 2^-39 of it; 22 bits of fp32 ones).
+template <typename QT, int D>
+struct HalfQuery {
+  static constexpr int kTerms = sizeof(QT) == 4 ? 2 : 1;
+  half8_t op[kTerms][D / 32];
+};
+
+// Builds the lane's query operand from its elements d = 16 qg + 64 h + [0, 16) and returns the
+// factor of its scores (NaN for a column that is not finite). Cross-lane.
+template <typename QT, int D>
+__device__ __forceinline__ float half_query(const QueryColumn<QT, D>& raw, bool valid, float scale,
+                                            HalfQuery<QT, D>& q) {
+  float x[D / 64][16];
+  float mx = 0.f;
+#pragma unroll
+  for (int h = 0; h < D / 64; ++h) {
+    const QT* e = reinterpret_cast<const QT*>(raw.w[h]);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      x[h][i] = valid ? to_float<QT>(e[i]) : 0.f;
+      mx = vmax(mx, fabsf(x[h][i]));  // NaN-propagating
+    }
+  }
+  mx = vmax(mx, shfl_xor(mx, 16));
+  mx = vmax(mx, shfl_xor(mx, 32));
+  const bool finite = __builtin_isfinite(mx);
+  int ex = 15;
+  if (finite && mx > 0.f) frexpf(mx, &ex);
+  ex = max(ex - 15, -126);
+#pragma unroll
+  for (int h = 0; h < D / 64; ++h)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float v = ldexpf(x[h][i], -ex);
+      const _Float16 hi = (_Float16)v;
+      q.op[0][2 * h + i / 8][i % 8] = hi;
+      if constexpr (HalfQuery<QT, D>::kTerms == 2)
+        q.op[1][2 * h + i / 8][i % 8] = (_Float16)(v - (float)hi);
+    }
+  return finite ? ldexpf(1.f, ex) * scale * code_scale<KF>() : __builtin_nanf("");
+}
+
+template <typename QT, int D>
+__device__ __forceinline__ float make_query(const QueryColumn<QT, D>& raw, bool valid, float scale,
+                                            QkOperand<D, kInt8>& q) {
+  return query_column_i8<QT, D>(raw, valid, scale, q.hi, q.lo, q.lo2);
+}
+template <typename QT, int D>
+__device__ __forceinline__ float make_query(const QueryColumn<QT, D>& raw, bool valid, float scale,
+                                            HalfQuery<QT, D>& q) {
+  return half_query<QT, D>(raw, valid, scale, q);
+}
+template <typename QT, int D>
+using QueryOp = std::conditional_t<KF == kInt8, QkOperand<D, kInt8>, HalfQuery<QT, D>>;
+
+// The unit 2^e of the V scales: weights enter the output's products as p * (v_scale * 2^-e)
+// in f16, the accumulators hold the output times 2^-e. The first block's largest scale sets
+// it to [2^4, 2^5) units, and a block with one above 2^7 sets it anew: p <= 2^kRescaleSlack
+// keeps the products' weights at 2^15 or less, and above f16's smallest step (2^-24) down to
+// 2^-28 of the largest.
+struct VUnit {
+  int e;
+  float inv, limit;
+};
+
+// One staged block through the MFMAs. Lane (qg, r) holds the scores of keys 4 qg + j for
+// head r; raw scores of keys outside [lo, hi) and of padding keys are -inf. `scores` (WEIGHTS):
+// where the lane's four scores go.
+template <typename QT, int D, bool WEIGHTS>
+__device__ __forceinline__ void bounded_block(const char* st, const QueryOp<QT, D>& q, float cf,
+                                              int tok_base, int lo, int hi, bool gvalid, int r,
+                                              int qg, float4_t (&acc)[D / 16], float& m, float& l,
+                                              VUnit& vu, bool& bad_score, bool masks,
+                                              float* scores) {
+  using S = Stage<D>;
+  constexpr int KCH = D / 64, VB = D / 16, NPV = D / 16;
+  const float4_t vs = *reinterpret_cast<const float4_t*>(st + S::kS + 64 + 16 * qg) * code_scale<KF>();
+  const float4_t ks = *reinterpret_cast<const float4_t*>(st + S::kS + 16 * qg);
+  const float screened = *reinterpret_cast<const float*>(st + S::kS + 64 + 4 * r);
+  float4_t s4;
+  if constexpr (KF == kInt8) {
+    int4_t si = {0, 0, 0, 0}, sf = {0, 0, 0, 0};
+    int4_t kop[KCH];
+#pragma unroll
+    for (int h = 0; h < KCH; ++h)
+      kop[h] = *reinterpret_cast<const int4_t*>(st + S::kK + k_chunk<D>(r, qg + 4 * h));
+#pragma unroll
+    for (int h = 0; h < KCH; ++h) si = __builtin_amdgcn_mfma_i32_16x16x64_i8(kop[h], q.hi[h], si, 0, 0, 0);
+#pragma unroll
+    for (int h = 0; h < KCH; ++h) sf = __builtin_amdgcn_mfma_i32_16x16x64_i8(kop[h], q.lo2[h], sf, 0, 0, 0);
+    si = si << 7;
+#pragma unroll
+    for (int h = 0; h < KCH; ++h) si = __builtin_amdgcn_mfma_i32_16x16x64_i8(kop[h], q.lo[h], si, 0, 0, 0);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s4[j] = __builtin_fmaf((float)sf[j], 1.f / 128.f, (float)si[j]);
+  } else {
+    s4 = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int h = 0; h < KCH; ++h) {
+      const uint4 c = *reinterpret_cast<const uint4*>(st + S::kK + k_chunk<D>(r, qg + 4 * h));
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub) {
+        half2_t p0, p1, p2, p3;
+        codes_to_f16<KF>(sub ? c.z : c.x, p0, p1);
+        codes_to_f16<KF>(sub ? c.w : c.y, p2, p3);
+        const half8_t kop = {p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
+#pragma unroll
+        for (int t = 0; t < HalfQuery<QT, D>::kTerms; ++t)
+          s4 = __builtin_amdgcn_mfma_f32_16x16x32_f16(kop, q.op[t][2 * h + sub], s4, 0, 0, 0);
+      }
+    }
+  }
+  // the conversions of MFMA results stay ahead of the branches below: sunk into their blocks,
+  // they have been issued without the wait states an MFMA result needs
+  asm volatile("" : "+v"(s4[0]), "+v"(s4[1]), "+v"(s4[2]), "+v"(s4[3]));
+
+  if (__builtin_expect(__ballot(screened * code_scale<KF>() > vu.limit) != 0, 0)) {
+    float top = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
+    top = fmaxf(top, shfl_xor(top, 16));
+    top = fmaxf(top, shfl_xor(top, 32));
+    int x = 5;
+    if (__builtin_isfinite(top) && top > 0.f) frexpf(top, &x);
+    x = min(max(x - 5, -120), 120);
+    const float down = ldexpf(1.f, max(vu.e - x, -250));  // (a first block's accumulators are 0)
+#pragma unroll
+    for (int n = 0; n < NPV; ++n) acc[n] *= down;
+    vu = VUnit{x, ldexpf(1.f, -x), ldexpf(1.f, x + 7)};
+  }
+
+  bool padded = false;
+  if (masks) padded = __ballot(*reinterpret_cast<const uint32_t*>(st + S::kF + 4 * qg) != 0x01010101u) != 0;
+  float sc[4];
+  bool nonfinite = false;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) sc[j] = s4[j] * (ks[j] * cf);
+  if (tok_base < lo || tok_base + kBlockTokens > hi || padded) {
+    const int tok0 = tok_base + 4 * qg;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool seen = tok0 + j >= lo && tok0 + j < hi && (!masks || st[S::kF + 4 * qg + j] != 0);
+      nonfinite |= gvalid && seen && !__builtin_isfinite(sc[j]);
+      sc[j] = seen ? sc[j] : -INFINITY;
+    }
+  } else {
+    const float most = vmax(vmax(sc[0], sc[1]), vmax(sc[2], sc[3]));
+    const float least = vmin(vmin(sc[0], sc[1]), vmin(sc[2], sc[3]));
+    nonfinite = gvalid && !(__builtin_isfinite(most) && __builtin_isfinite(least));
+  }
+  if (__builtin_expect(__ballot(nonfinite) != 0, 0)) bad_score = true;
+  float tmax = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
+  if (__builtin_expect(__ballot(gvalid && tmax > m + kRescaleSlack) != 0, 0)) {
+    tmax = fmaxf(tmax, shfl_xor(tmax, 16));
+    tmax = fmaxf(tmax, shfl_xor(tmax, 32));
+    const float mn = fmaxf(m, tmax);
+    const float alpha = __builtin_amdgcn_exp2f(m - mn);
+    l *= alpha;
+#pragma unroll
+    for (int n = 0; n < NPV; ++n) acc[n] *= alpha;
+    m = mn;
+  }
+  if constexpr (WEIGHTS) {
+    if (gvalid) *reinterpret_cast<float4_t*>(scores) = float4_t{sc[0], sc[1], sc[2], sc[3]};
+  }
+  constexpr int kTerms = sizeof(QT) == 4 ? 2 : 1;
+  half4_t pop[kTerms];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float p = __builtin_amdgcn_exp2f(sc[j] - m);
+    l += p;
+    float w = p * (vs[j] * vu.inv);
+    // (one rounding of the product for both terms: a multiply that rounds to f16 by itself would
+    // now and then give a first term that the second does not fit)
+    if constexpr (kTerms == 2) asm volatile("" : "+v"(w));
+    pop[0][j] = (_Float16)w;
+    if constexpr (kTerms == 2) pop[1][j] = (_Float16)(w - (float)pop[0][j]);
+  }
+  uint32_t vw[4][VB / 4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const char* rowp = st + S::kV + (4 * qg + j) * D + r * VB;
+    struct alignas(VB) Run {
+      uint32_t w[VB / 4];
+    };
+    const Run run = *reinterpret_cast<const Run*>(rowp);
+#pragma unroll
+    for (int i = 0; i < VB / 4; ++i) vw[j][i] = run.w[i];
+  }
+  // O^T += V^T P^T (row i of MFMA n is d = VB i + n)
+#pragma unroll
+  for (int n = 0; n < NPV; ++n) {
+    const uint32_t col[4] = {vw[0][n / 4], vw[1][n / 4], vw[2][n / 4], vw[3][n / 4]};
+    half4_t vop;
+    switch (n % 4) {
+      case 0: vop = v_operand<0, KF>(col); break;
+      case 1: vop = v_operand<1, KF>(col); break;
+      case 2: vop = v_operand<2, KF>(col); break;
+      default: vop = v_operand<3, KF>(col); break;
+    }
+#pragma unroll
+    for (int t = 0; t < kTerms; ++t)
+      acc[n] = __builtin_amdgcn_mfma_f32_16x16x16f16(vop, pop[t], acc[n], 0, 0, 0);
+  }
+}
+
+// Adds the weights of keys [t0, t1) of one (sequence, KV head): its scores (base 2) at
+// `scores` (one row per head, a.score_stride apart), lse (base 2) of its heads in `lse`. The
+// row's newest key starts at 0.
+__device__ __forceinline__ void add_weights(const BoundedArgs& a, const float* scores,
+                                            const float* lse, float* weights, int ctx, int t0,
+                                            int t1, int thread, int threads) {
+  const int G = a.group;
+  t1 = min(t1, min(ctx, a.kw.capacity));
+  for (int t = t0 + 4 * thread; t < t1; t += 4 * threads) {
+    float4_t sum = {0.f, 0.f, 0.f, 0.f};
+    for (int g = 0; g < G; ++g) {
+      const float4_t s = *reinterpret_cast<const float4_t*>(scores + g * a.score_stride + t);
+      const float e = lse[g];
+      if (e == INFINITY) continue;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum[j] += __builtin_amdgcn_exp2f(s[j] - e);
+    }
+    if (t + 4 <= min(t1, ctx - 1)) {
+      *reinterpret_cast<float4_t*>(weights + t) += sum;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (t + j < t1) weights[t + j] = (t + j == ctx - 1 ? 0.f : weights[t + j]) + sum[j];
+    }
+  }
+}
+
+__device__ __forceinline__ int row_parts(const BoundedArgs& a, const VisibleList& v) {
+  const int parts = (v.blocks + a.part_blocks - 1) / a.part_blocks;
+  return parts < 1 ? 1 : parts;  // <= max_parts: v comes of a length within max_context
+}
+
+// log2 of the sum over keys; +inf where the head saw none or its scores are not finite: it
+// adds no weights.
+__device__ __forceinline__ float log_sum(float m, float l) {
+  return l > 0.f ? m + __builtin_amdgcn_logf(l) : INFINITY;
+}
+
+template <int D, int NW>
+struct BoundedLds {
+  static constexpr int kStageBytes = NW * Stage<D>::kBytes;
+  static constexpr int kMergeBytes = NW * 16 * (D + 2) * 4;
+  static constexpr int kBytes = 2 * kStageBytes > kMergeBytes ? 2 * kStageBytes : kMergeBytes;
+};
+
+template <typename QT, int D, int NW, bool WEIGHTS>
+__global__ __launch_bounds__(NW * kWave) void bounded_decode_kernel(BoundedArgs a) {
+  static_assert(D == 64 || D == 128 || D == 256, "head_dim");
+  using S = Stage<D>;
+  using L = BoundedLds<D, NW>;
+  constexpr int NPV = D / 16, VB = D / 16;
+  __shared__ __attribute__((aligned(16))) char lds[L::kBytes];
+  __shared__ float lse[16];
+
+  const int part = blockIdx.x, kvh = blockIdx.y, seq = blockIdx.z;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int lane = threadIdx.x % kWave;
+  const int r = lane & 15, qg = lane >> 4;
+  const int G = a.group;
+  const bool gvalid = r < G;
+  const int tok = decode_token(a, seq);
+  if (tok < 0) return;  // not a decode row
+  QueryColumn<QT, D> raw;
+  load_query_column<QT, D>(query_col_ptr<QT>(a, tok, kvh * G + (gvalid ? r : 0), qg), raw);
+  const bool reporter = part == 0 && kvh == 0 && threadIdx.x == 0;
+  const VisibleList v = visible_list(a, bounded_ctx(a, a.context_lens[seq], reporter));
+  const int parts = row_parts(a, v);
+  if (part >= parts) return;
+  const int f0 = part * a.part_blocks + wave;
+  const int f1 = min(v.blocks, (part + 1) * a.part_blocks);
+  const int nbw = f0 < f1 ? (f1 - f0 + NW - 1) / NW : 0;  // at most 64 (host)
+  const int32_t* bt = a.block_tables + (int64_t)seq * a.bt_stride;
+  const int ids = lane < nbw ? bt[v.block(f0 + NW * lane)] : 0;
+  // a block outside the arena: the wave reports it and reads nothing
+  const bool bad_index = __ballot(lane < nbw && (unsigned)ids >= (unsigned)a.cache.num_blocks) != 0;
+  const int nblk = bad_index ? 0 : nbw;
+
+  char* const st0 = lds + wave * S::kBytes;
+  char* const st1 = lds + L::kStageBytes + wave * S::kBytes;
+  if (0 < nblk) stage_block<D>(a, __builtin_amdgcn_readlane(ids, 0), kvh, lane, st0);
+  if (1 < nblk) stage_block<D>(a, __builtin_amdgcn_readlane(ids, 1), kvh, lane, st1);
+
+  QueryOp<QT, D> q;
+  const float cf = make_query<QT, D>(raw, gvalid, a.qk_scale_log2, q);
+  float4_t acc[NPV];
+#pragma unroll
+  for (int n = 0; n < NPV; ++n) acc[n] = float4_t{0.f, 0.f, 0.f, 0.f};
+  float m = gvalid ? -FLT_MAX : 0.f, l = 0.f;  // finite: a block without a visible key adds 0
+  VUnit vu{0, 1.f, -1.f};
+  bool bad_score = false;
+  const bool masks = a.cache.key_valid != nullptr;
+  const int64_t unit = (int64_t)seq * a.cache.num_kv_heads + kvh;
+  float* const srow = WEIGHTS ? a.scores + (unit * G + (gvalid ? r : 0)) * a.score_stride : nullptr;
+
+  auto step = [&](int i, char* st) __attribute__((always_inline)) {
+    // block i has landed once only the next one's loads may be on their way (loads complete in
+    // order; a padding load or a score store among the younger ones makes this wait longer)
+    if (i + 1 < nblk) wait_vmcnt<S::kLoads>();
+    else wait_vmcnt<0>();
+    const int f = f0 + NW * i;
+    const int base = v.block(f) * kBlockTokens;
+    bounded_block<QT, D, WEIGHTS>(st, q, cf, base, v.lo(f), v.hi(f), gvalid, r, qg, acc, m, l, vu,
+                                  bad_score, masks, WEIGHTS ? srow + base + 4 * qg : nullptr);
+    if (i + 2 < nblk) stage_block<D>(a, __builtin_amdgcn_readlane(ids, i + 2), kvh, lane, st);
+  };
+  for (int i = 0; i < nblk; i += 2) {
+    step(i, st0);
+    if (i + 1 >= nblk) break;
+    step(i + 1, st1);
+  }
+  if (bad_index) {
+    if (lane == 0) atomicOr(a.err_flag, ASTR_FLAG_BAD_INDEX);
+    if (WEIGHTS && gvalid)  // its keys add no weight
+      for (int i = 0; i < nbw; ++i)
+        *reinterpret_cast<float4_t*>(srow + v.block(f0 + NW * i) * kBlockTokens + 4 * qg) =
+            float4_t{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  }
+  if (bad_score && lane == 0) atomicOr(a.err_flag, ASTR_FLAG_NONFINITE_SCORE);
+
+  // ---- the waves' states, in LDS (over the stages: every wave has read its own)
+  l += shfl_xor(l, 16);
+  l += shfl_xor(l, 32);
+  const float up = ldexpf(1.f, vu.e);
+  __syncthreads();
+  float* const sm = reinterpret_cast<float*>(lds);  // [NW][16]
+  float* const sl = sm + NW * 16;
+  float* const so = sl + NW * 16;  // [NW][G][D]
+  if (gvalid) {
+    if (qg == 0) {
+      sm[wave * 16 + r] = m;
+      sl[wave * 16 + r] = l;
+    }
+    float* o = so + (wave * G + r) * D + VB * 4 * qg;
+#pragma unroll
+    for (int n = 0; n < NPV; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[VB * j + n] = acc[n][j] * up;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < G * D; i += NW * kWave) {
+    const int g = i / D, d = i % D;
+    float M = -FLT_MAX;
+    for (int w = 0; w < NW; ++w) M = fmaxf(M, sm[w * 16 + g]);
+    float Lg = 0.f, O = 0.f;
+    for (int w = 0; w < NW; ++w) {
+      const float f = __builtin_amdgcn_exp2f(sm[w * 16 + g] - M);
+      Lg = fmaf(sl[w * 16 + g], f, Lg);
+      O = fmaf(so[(w * G + g) * D + d], f, O);
+    }
+    const int h = kvh * G + g;
+    if (parts == 1) {
+      static_cast<QT*>(a.out)[(int64_t)tok * a.o_tok + (int64_t)h * a.o_head + d] =
+          from_float<QT>(O / fmaxf(Lg, FLT_MIN));
+      if (WEIGHTS && d == 0) lse[g] = log_sum(M, Lg);
+    } else {
+      const int64_t at = ((int64_t)seq * a.num_q_heads + h) * a.max_parts + part;
+      a.ws_o[at * D + d] = O;
+      if (d == 0) {
+        a.ws_ml[at * 2] = M;
+        a.ws_ml[at * 2 + 1] = Lg;
+      }
+    }
+  }
+  if constexpr (WEIGHTS) {
+    if (parts > 1) return;
+    const int64_t row = weight_row(a, seq, reporter);
+    if (reporter && v.ctx > a.kw.capacity) atomicOr(a.err_flag, ASTR_FLAG_BAD_INDEX);
+    __threadfence_block();  // the scores, which other waves of the workgroup stored
+    __syncthreads();
+    if (row >= 0)
+      add_weights(a, a.scores + unit * G * a.score_stride, lse,
+                  a.kw.values + row * a.kw.row_stride + kvh * a.kw.head_stride, v.ctx, 0, v.ctx,
+                  threadIdx.x, NW * kWave);
+  }
+}
+
+// The second launch, for rows of several pieces: the pieces' states merged into the output
+// (the first workgroup of a (sequence, KV head)), and the weights of kTileTokens keys each.
+template <typename QT, int D, bool WEIGHTS>
+__global__ __launch_bounds__(256) void bounded_merge_kernel(BoundedArgs a) {
+  __shared__ float top[16], sum[16], lse[16];
+  const int tile = blockIdx.x, kvh = blockIdx.y, seq = blockIdx.z;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int lane = threadIdx.x % kWave;
+  const int tok = decode_token(a, seq);
+  if (tok < 0) return;
+  const VisibleList v = visible_list(a, bounded_ctx(a, a.context_lens[seq], false));
+  const int parts = row_parts(a, v);
+  if (parts <= 1 || (tile > 0 && tile * kTileTokens >= v.ctx)) return;
+  const int G = a.group;
+  const int64_t head0 = (int64_t)seq * a.num_q_heads + kvh * G;
+  for (int g = wave; g < G; g += kWaves) {
+    const float* ml = a.ws_ml + (head0 + g) * a.max_parts * 2;
+    float M = -FLT_MAX;
+    for (int p = lane; p < parts; p += kWave) M = fmaxf(M, ml[2 * p]);
+    M = wave_max(M);
+    float Lg = 0.f;
+    for (int p = lane; p < parts; p += kWave)
+      Lg = fmaf(ml[2 * p + 1], __builtin_amdgcn_exp2f(ml[2 * p] - M), Lg);
+    Lg = wave_sum(Lg);
+    if (lane == 0) {
+      top[g] = M;
+      sum[g] = Lg;
+      lse[g] = log_sum(M, Lg);
+    }
+  }
+  __syncthreads();
+  if (tile == 0) {
+    for (int i = threadIdx.x; i < G * D; i += 256) {
+      const int g = i / D, d = i % D;
+      const int64_t at = (head0 + g) * a.max_parts;
+      float O = 0.f;
+#pragma unroll 4
+      for (int p = 0; p < parts; ++p)
+        O = fmaf(a.ws_o[(at + p) * D + d], __builtin_amdgcn_exp2f(a.ws_ml[(at + p) * 2] - top[g]), O);
+      static_cast<QT*>(a.out)[(int64_t)tok * a.o_tok + (int64_t)(kvh * G + g) * a.o_head + d] =
+          from_float<QT>(O / fmaxf(sum[g], FLT_MIN));
+    }
+  }
+  if constexpr (WEIGHTS) {
+    const bool reporter = tile == 0 && kvh == 0 && threadIdx.x == 0;
+    const int64_t row = weight_row(a, seq, reporter);
+    if (reporter && v.ctx > a.kw.capacity) atomicOr(a.err_flag, ASTR_FLAG_BAD_INDEX);
+    if (row >= 0)
+      add_weights(a, a.scores + ((int64_t)seq * a.cache.num_kv_heads + kvh) * G * a.score_stride,
+                  lse, a.kw.values + row * a.kw.row_stride + kvh * a.kw.head_stride, v.ctx,
+                  tile * kTileTokens, (tile + 1) * kTileTokens, threadIdx.x, 256);
+  }
+}
+
+template <typename QT, int D, int NW, bool WEIGHTS>
+int launch(const BoundedArgs& a, hipStream_t stream) {
+  const dim3 grid((uint32_t)a.max_parts, (uint32_t)a.cache.num_kv_heads, (uint32_t)a.num_seqs);
+  hipLaunchKernelGGL((bounded_decode_kernel<QT, D, NW, WEIGHTS>), grid, dim3(NW * kWave), 0, stream, a);
+  if (a.max_parts > 1) {
+    const int tiles = WEIGHTS ? (a.max_context + kTileTokens - 1) / kTileTokens : 1;
+    hipLaunchKernelGGL((bounded_merge_kernel<QT, D, WEIGHTS>), dim3((uint32_t)tiles, grid.y, grid.z),
+                       dim3(256), 0, stream, a);
+  }
+  const hipError_t err = hipGetLastError();
+  return err == hipSuccess ? 0 : hip_fail(err, "paged_attention (bounded decode) launch");
+}
+
+template <typename QT, int D>
+int launch_dim(const BoundedArgs& a, hipStream_t s) {
+  const bool weights = a.kw.values != nullptr;
+  constexpr int W = wide_waves(D);
+  // total_waves: the workgroup's waves, four or wide_waves()
+  if (a.total_waves == W) return weights ? launch<QT, D, W, true>(a, s) : launch<QT, D, W, false>(a, s);
+  return weights ? launch<QT, D, 4, true>(a, s) : launch<QT, D, 4, false>(a, s);
+}
+
+template <typename QT>
+int launch_type(const BoundedArgs& a, hipStream_t s) {
+  switch (a.cache.head_dim) {
+    case 64: return launch_dim<QT, 64>(a, s);
+    case 128: return launch_dim<QT, 128>(a, s);
+    case 256: return launch_dim<QT, 256>(a, s);
+    default: return fail(ASTR_EUNSUPPORTED, "head_dim %d not in {64,128,256}", a.cache.head_dim);
+  }
+}
+
+}  // namespace
+
+template <>
+int launch_bounded_kf<KF>(const BoundedArgs& a, int32_t q_dtype, hipStream_t stream) {
+  switch (q_dtype) {
+    case ASTR_F32: return launch_type<float>(a, stream);
+    case ASTR_F16: return launch_type<_Float16>(a, stream);
+    default: return launch_type<bf16_t>(a, stream);
+  }
+}
+
+}  // namespace attn
+}  // namespace astr

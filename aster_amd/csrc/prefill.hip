@@ -25,12 +25,15 @@
 // and the linear workgroup id is remapped so that each XCD (workgroups are dealt
 // to the 8 XCDs round robin) runs one contiguous range of units: the tiles
 // sharing a sequence's K/V then share that XCD's L2.
+//
+// Built once more with -DASTR_PF_SINKS=1: the first `sinks` keys stay visible beside the
+// window. A unit's blocks of sinks below its window run first, as key steps of their own.
 #include <algorithm>
 #include <climits>
 #include <cstddef>
 #include <type_traits>
 
-#include "attention_common.h"
+#include "bounded_common.h"
 
 namespace astr {
 namespace attn {
@@ -40,6 +43,17 @@ namespace {
 #define ASTR_KF 0
 #endif
 constexpr int KF = ASTR_KF;  // this translation unit's code format
+
+#ifndef ASTR_PF_SINKS
+#define ASTR_PF_SINKS 0
+#endif
+constexpr bool kSinks = ASTR_PF_SINKS != 0;
+// The kernels' arguments. sinks_of is 0 without sinks, which leaves no code.
+using PrefillArgs = std::conditional_t<kSinks, SinkChunkArgs, ChunkArgs>;
+__host__ __device__ __forceinline__ int sinks_of(const ChunkArgs& a) {
+  if constexpr (kSinks) return static_cast<const SinkChunkArgs&>(a).sinks;
+  else return 0;
+}
 
 constexpr int kXcds = 8;
 
@@ -93,6 +107,22 @@ __device__ __forceinline__ TileSpan tile_span(const AttnArgs& a, int ctx, int n,
   t.b_lo = t.lo / kBlockTokens;
   t.b_hi = t.hi >= t.lo ? t.hi / kBlockTokens + 1 : t.b_lo;  // exclusive
   return t;
+}
+
+// With sinks: the blocks [0, n) of sinks below a tile's first window block, and the key steps
+// they take ahead of the window's. (A window block that holds sinks too shows them by the
+// bounds of its keys.)
+struct SinkSpan {
+  int blocks, steps, keys;
+};
+__device__ __forceinline__ SinkSpan sink_span(const ChunkArgs& a, const TileSpan& t) {
+  const int n = min((sinks_of(a) + kBlockTokens - 1) / kBlockTokens, t.b_lo);
+  return SinkSpan{n, (n + kWaves - 1) / kWaves, sinks_of(a)};
+}
+__device__ __forceinline__ int tile_steps(const ChunkArgs& a, const TileSpan& t) {
+  const int steps = (t.b_hi - t.b_lo + kWaves - 1) / kWaves;
+  if constexpr (kSinks) return steps + sink_span(a, t).steps;
+  return steps;
 }
 
 constexpr int kOrderMax = 256;  // chunk rows ordered longest first; beyond this, index order
@@ -533,7 +563,8 @@ __device__ __forceinline__ void prefill_half(const PrefillLds<D>& L, int buf, in
                                              uint32_t bounded, bool masks, int kb0,
                                              half8_t (&kop)[D / 16], Between between,
                                              const QOp<QT, D> (&qop)[NT], const float (&back)[NT],
-                                             const int (&lo)[NT], const int (&hi)[NT], int lane,
+                                             const int (&lo)[NT], const int (&hi)[NT], int sinks,
+                                             int lane,
                                              bool vmix, half2_t vf,
                                              float16v_t (&acc)[NT][D / 32], float (&m)[NT],
                                              float (&l)[NT], bool& bad_score) {
@@ -621,7 +652,9 @@ __device__ __forceinline__ void prefill_half(const PrefillLds<D>& L, int buf, in
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
             // -1 when key < lo or key > hi (either difference negative), else 0
-            const int32_t outside = bnd ? ((key - lo[t]) | (hi[t] - key)) >> 31 : 0;
+            // (a sink, key < sinks, is not below lo)
+            const int32_t below = kSinks ? (key - lo[t]) & ~(key - sinks) : key - lo[t];
+            const int32_t outside = bnd ? (below | (hi[t] - key)) >> 31 : 0;
             const uint32_t hide = used ? (uint32_t)(outside | padding) : 0xffffffffu;
             // (the factors first: a large query's beside a small key's stays in range)
             const uint32_t xb = __builtin_bit_cast(uint32_t, s[t][j] * (back[t] * ks[x][y]));
@@ -763,7 +796,9 @@ template <typename QT, int D, int KS, typename ColumnOf, typename BoundsOf, type
 __device__ __forceinline__ void prefill_unit(const AttnArgs& a, PrefillLds<D>& L, int kvh,
                                              int b_lo, int b_hi, const int32_t* blocks, int q0,
                                              int t0, ColumnOf column_of, BoundsOf bounds_of,
-                                             Store store, Prologue prologue, Mark mark) {
+                                             Store store, Prologue prologue, Mark mark,
+                                             SinkSpan sink = SinkSpan{0, 0, 0}, int step0 = 0,
+                                             int all_steps = 0) {
   using Shape = PrefillShape<D, KS>;
   constexpr int NT = Shape::NT;
   constexpr int kRowsN = D / 32;
@@ -771,14 +806,23 @@ __device__ __forceinline__ void prefill_unit(const AttnArgs& a, PrefillLds<D>& L
   const int lane = threadIdx.x % kWave;
   const int group = KS == 1 ? wave : wave % Shape::kGroups;
   const int half = KS == 1 ? 0 : wave / Shape::kGroups;
-  const int nsteps = (b_hi - b_lo + kWaves - 1) / kWaves;
+  // with sinks: the unit's steps [step0, step0 + nsteps) of those of its sink and window blocks
+  const int nsteps = kSinks ? all_steps : (b_hi - b_lo + kWaves - 1) / kWaves;
+  auto step_block = [&](int step) __attribute__((always_inline)) -> int {
+    if constexpr (!kSinks) return b_lo + step * kWaves;
+    const int j = step0 + step - sink.steps;
+    return j < 0 ? (step0 + step) * kWaves : b_lo + j * kWaves;
+  };
+  auto step_end = [&](int step) __attribute__((always_inline)) -> int {
+    return kSinks && step0 + step < sink.steps ? sink.blocks : b_hi;
+  };
 
   // Block b_lo + 4 * step + w is wave w's; its id is read (a scalar load) one step before
   // its block. A block past the range repeats the last one (its keys are not used).
   typedef const __attribute__((address_space(4))) int32_t* scalar_ids_t;
   const scalar_ids_t sids = (scalar_ids_t)blocks;
   auto id_of = [&](int step) __attribute__((always_inline)) -> int {
-    return sids[min(b_lo + step * kWaves + wave, b_hi - 1)];
+    return sids[min(step_block(step) + wave, step_end(step) - 1)];
   };
   int next_id = nsteps > 0 ? id_of(0) : 0;
   __syncthreads();  // what the stage memory held before (the dispatch plan) has been read
@@ -882,17 +926,19 @@ __device__ __forceinline__ void prefill_unit(const AttnArgs& a, PrefillLds<D>& L
         vf[w] = (_Float16)ldexpf(1.f, e4[w] - ve);
       }
     }
-    const int kb0 = (b_lo + i * kWaves) * kBlockTokens;
+    const int kb0 = step_block(i) * kBlockTokens;
+    const int wi = kSinks ? step0 + i - sink.steps : i;  // the window's step
     uint32_t use = 15, bounded = 0;
-    if (i < inner_lo || i >= inner_hi) {
-      const int kend = b_hi * kBlockTokens;
+    if (wi < inner_lo || wi >= inner_hi) {
+      const int kend = step_end(i) * kBlockTokens;
       use = 0;
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) {
         const int kb = kb0 + w * kBlockTokens;
-        if (wb.any && kb < kend && kb <= wb.hi_max && kb + kBlockTokens - 1 >= wb.lo_min)
+        const bool some = kSinks && kb < sink.keys, all = kSinks && kb + kBlockTokens <= sink.keys;
+        if (wb.any && kb < kend && kb <= wb.hi_max && (kb + kBlockTokens - 1 >= wb.lo_min || some))
           use |= 1u << w;
-        if (!(kb >= wb.lo_max && kb + kBlockTokens - 1 <= wb.hi_min)) bounded |= 1u << w;
+        if (!((kb >= wb.lo_max || all) && kb + kBlockTokens - 1 <= wb.hi_min)) bounded |= 1u << w;
       }
       bounded &= use;
     }
@@ -900,7 +946,7 @@ __device__ __forceinline__ void prefill_unit(const AttnArgs& a, PrefillLds<D>& L
       const uint32_t mine = use >> (2 * half) & 3u;
       if (mine != 0)
         prefill_half<QT, D, NT>(L, buf, half, mine | slow, bounded >> (2 * half) & 3u, masks,
-                                kb0 + 32 * half, kop, []() {}, qop, back, lo, hi, lane, vmix,
+                                kb0 + 32 * half, kop, []() {}, qop, back, lo, hi, sink.keys, lane, vmix,
                                 half != 0 ? half2_t{vf[2], vf[3]} : half2_t{vf[0], vf[1]}, acc, m,
                                 l, bad_score);
     } else if (use != 0) {
@@ -908,10 +954,10 @@ __device__ __forceinline__ void prefill_unit(const AttnArgs& a, PrefillLds<D>& L
                               [&]() __attribute__((always_inline)) {
                                 load_k_operands<D>(L, buf, 1, lane, kop);
                               },
-                              qop, back, lo, hi, lane, vmix, half2_t{vf[0], vf[1]}, acc, m, l,
-                              bad_score);
+                              qop, back, lo, hi, sink.keys, lane, vmix, half2_t{vf[0], vf[1]}, acc, m,
+                              l, bad_score);
       prefill_half<QT, D, NT>(L, buf, 1, use >> 2 | slow, bounded >> 2, masks, kb0 + 32, kop,
-                              []() {}, qop, back, lo, hi, lane, vmix, half2_t{vf[2], vf[3]}, acc,
+                              []() {}, qop, back, lo, hi, sink.keys, lane, vmix, half2_t{vf[2], vf[3]}, acc,
                               m, l, bad_score);
     }
     if (i + 1 < nsteps) {
@@ -1049,7 +1095,7 @@ __device__ __forceinline__ void store_column(const AttnArgs& a, const float16v_t
 }
 
 template <typename QT, int D, int G, int KS>
-__global__ __launch_bounds__(256, (prefill_occupancy<QT, D>())) void prefill_mfma_kernel(ChunkArgs a) {
+__global__ __launch_bounds__(256, (prefill_occupancy<QT, D>())) void prefill_mfma_kernel(PrefillArgs a) {
   static_assert(D == 64 || D == 128 || D == 256, "head_dim");
   constexpr int NT = PrefillShape<D, KS>::NT;
   constexpr int TQ = PrefillShape<D, KS>::kCols / G;
@@ -1101,8 +1147,9 @@ __global__ __launch_bounds__(256, (prefill_occupancy<QT, D>())) void prefill_mfm
   const int pos0 = span.pos0, t0 = span.t0, t1 = span.t1;
   // the piece's key steps; a unit within pf_steps is its first piece alone
   float* part = nullptr;
+  int step0 = 0, nsteps = kSinks ? tile_steps(a, span) : 0;
   if (a.pf_pieces > 1) {
-    const int steps = (span.b_hi - span.b_lo + kWaves - 1) / kWaves;
+    const int steps = tile_steps(a, span);
     if (piece > 0 && piece * a.pf_steps >= steps) return;
     if (steps > a.pf_steps) {
       if ((uint64_t)(logical + 1) * PiecePartial<D, KS>::kFloats * sizeof(float) > a.pf_bytes) {
@@ -1110,9 +1157,14 @@ __global__ __launch_bounds__(256, (prefill_occupancy<QT, D>())) void prefill_mfm
         return;
       }
       part = a.pf_ws + logical * PiecePartial<D, KS>::kFloats;
-      span.b_lo += piece * a.pf_steps * kWaves;
       // (the last piece takes whatever a context past the host's bound adds)
-      if (piece < a.pf_pieces - 1) span.b_hi = min(span.b_hi, span.b_lo + a.pf_steps * kWaves);
+      if constexpr (kSinks) {
+        step0 = piece * a.pf_steps;
+        nsteps = piece < a.pf_pieces - 1 ? min(a.pf_steps, steps - step0) : steps - step0;
+      } else {
+        span.b_lo += piece * a.pf_steps * kWaves;
+        if (piece < a.pf_pieces - 1) span.b_hi = min(span.b_hi, span.b_lo + a.pf_steps * kWaves);
+      }
     }
   }
 
@@ -1155,7 +1207,8 @@ __global__ __launch_bounds__(256, (prefill_occupancy<QT, D>())) void prefill_mfm
   };
   prefill_unit<QT, D, KS>(a, L, kvh, span.b_lo, span.b_hi,
                       a.block_tables + (int64_t)seq * a.bt_stride, q0, t0, column_of,
-                      bounds_of, store, []() { return true; }, [](int) {});
+                      bounds_of, store, []() { return true; }, [](int) {}, sink_span(a, span),
+                      step0, nsteps);
 }
 
 constexpr int kMostPieces = 16;
@@ -1177,7 +1230,7 @@ struct MergeShape {
 };
 
 template <typename QT, int D, int G, int KS>
-__global__ __launch_bounds__(256) void prefill_merge_kernel(ChunkArgs a) {
+__global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillArgs a) {
   using Shape = PrefillShape<D, KS>;
   using Partial = PiecePartial<D, KS>;
   using M = MergeShape<D>;
@@ -1218,7 +1271,7 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(ChunkArgs a) {
   UnitRef u;
   if (!unit_ref(a, TQ, tab, s_wsum, s_found, rows, unit % per_kv, u)) return;
   const TileSpan span = tile_span(a, clamp_ctx(a, u.ctx_raw, false), u.n, u.tile, TQ);
-  const int steps = (span.b_hi - span.b_lo + kWaves - 1) / kWaves;
+  const int steps = tile_steps(a, span);
   const int pieces = min((steps + a.pf_steps - 1) / a.pf_steps, a.pf_pieces);
   if (pieces <= 1) return;
   float mx = -FLT_MAX;
@@ -1265,6 +1318,7 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(ChunkArgs a) {
 // the member row's chunk slot, for the chunk-merge kernel (decode_planned.hip) to merge
 // with the row's other ranges and its own blocks. Tiles reading the same blocks (one kv
 // head and range) are consecutive and run on one XCD, whose L2 then serves their keys.
+#if !ASTR_PF_SINKS
 constexpr int kTileWords = 8, kMemberWords = 3;
 
 template <typename QT, int D, int G>
@@ -1421,6 +1475,8 @@ __global__ __launch_bounds__(256, (prefill_occupancy<QT, D>())) void prefix_tile
 #endif
 }
 
+#endif  // !ASTR_PF_SINKS
+
 // Compute units of the current device (256 where that cannot be read).
 int prefill_cus() {
   int dev = 0, v = 0;
@@ -1458,10 +1514,11 @@ struct Split {
   int64_t time;           // of the longest unit (step_time, kSplitTime)
 };
 template <typename QT, int D, int G, int KS>
-Split key_split(const ChunkArgs& a, int cus) {
+Split key_split(const PrefillArgs& a, int cus) {
   constexpr int TQ = PrefillShape<D, KS>::kCols / G;
   int64_t keys = a.max_context;
   if (a.window > 0) keys = std::min<int64_t>(keys, (int64_t)a.window + TQ + kBlockTokens);
+  if constexpr (kSinks) keys += sinks_of(a) + kWaves * kBlockTokens;  // (its steps round up apart)
   const int64_t steps = (keys + kWaves * kBlockTokens - 1) / (kWaves * kBlockTokens) + 1;
   const int64_t room = (int64_t)(a.pf_bytes / (PiecePartial<D, KS>::kFloats * sizeof(float)));
   const int64_t resident = (int64_t)cus * prefill_occupancy<QT, D>();
@@ -1476,7 +1533,7 @@ Split key_split(const ChunkArgs& a, int cus) {
 }
 
 template <typename QT, int D, int G, int KS>
-int launch_shape(ChunkArgs a, const Split& split, int cus, hipStream_t stream) {
+int launch_shape(PrefillArgs a, const Split& split, int cus, hipStream_t stream) {
   a.pf_cus = cus >= kXcds ? cus / kXcds : 1;
   a.pf_pieces = split.pieces;
   a.pf_steps = split.steps;
@@ -1498,7 +1555,7 @@ int launch_shape(ChunkArgs a, const Split& split, int cus, hipStream_t stream) {
 // heads) stay with KS = 1 and 8 pieces, 75.8 us. Past the GPU's CUs its units queue: 1500 tokens
 // (16/4 heads) 86.5 us with KS = 1, 96.8 with KS = 2.
 template <typename QT, int D, int G>
-int launch(const ChunkArgs& a, hipStream_t stream) {
+int launch(const PrefillArgs& a, hipStream_t stream) {
   const int cus = prefill_cus();
   const Split whole = key_split<QT, D, G, 1>(a, cus);
   if (whole.units == 0) return 0;
@@ -1511,7 +1568,7 @@ int launch(const ChunkArgs& a, hipStream_t stream) {
 }
 
 template <typename QT, int D>
-int dispatch_group(const ChunkArgs& a, int G, hipStream_t s) {
+int dispatch_group(const PrefillArgs& a, int G, hipStream_t s) {
   switch (G) {
     case 1: return launch<QT, D, 1>(a, s);
     case 2: return launch<QT, D, 2>(a, s);
@@ -1523,7 +1580,7 @@ int dispatch_group(const ChunkArgs& a, int G, hipStream_t s) {
 }
 
 template <typename QT>
-int dispatch_dim(const ChunkArgs& a, int G, hipStream_t s) {
+int dispatch_dim(const PrefillArgs& a, int G, hipStream_t s) {
   switch (a.cache.head_dim) {
     case 64: return dispatch_group<QT, 64>(a, G, s);
     case 128: return dispatch_group<QT, 128>(a, G, s);
@@ -1532,6 +1589,7 @@ int dispatch_dim(const ChunkArgs& a, int G, hipStream_t s) {
   }
 }
 
+#if !ASTR_PF_SINKS
 template <typename QT, int D, int G>
 int launch_tiles(const PlanArgs& p, hipStream_t stream) {
   const int64_t grid = ((int64_t)p.info.num_tiles + kXcds - 1) / kXcds * kXcds;
@@ -1565,8 +1623,21 @@ int tiles_dim(const PlanArgs& p, int G, hipStream_t s) {
   }
 }
 
+#endif  // !ASTR_PF_SINKS
+
 }  // namespace
 
+#if ASTR_PF_SINKS
+template <>
+int launch_prefill_sinks_kf<KF>(const SinkChunkArgs& a, int32_t q_dtype, hipStream_t stream) {
+  const int G = a.num_q_heads / a.cache.num_kv_heads;
+  switch (q_dtype) {
+    case ASTR_F32: return dispatch_dim<float>(a, G, stream);
+    case ASTR_F16: return dispatch_dim<_Float16>(a, G, stream);
+    default: return dispatch_dim<bf16_t>(a, G, stream);
+  }
+}
+#else
 #if ASTR_TRACE && ASTR_KF == 0
 // Trace builds: copies the marks and info of the first `waves` waves of the last
 // prefix-tile launch of the int8 format (8 int64 + 4 int32 per wave; wave w of tile
@@ -1598,6 +1669,7 @@ int launch_prefill_kf<KF>(const ChunkArgs& a, int32_t q_dtype, hipStream_t strea
     default: return dispatch_dim<bf16_t>(a, G, stream);
   }
 }
+#endif  // ASTR_PF_SINKS
 
 }  // namespace attn
 }  // namespace astr

@@ -34,6 +34,7 @@ import torch
 
 from . import _native
 from .attention_backend import BACKEND, KernelWork, UnsupportedAttentionBackend
+from .key_weights import EvictedTokens, require_rows
 from .kv_quantization import KVQuantization, QuantizedKV, _DTYPE_CODES, require_format
 
 DEFAULT_PARTITION_TOKENS = 0  # automatic: stream-K for bf16/fp16, else 512-token partitions
@@ -308,7 +309,7 @@ class PagedKVCache:
                         scale=None, window=None, partition_tokens=DEFAULT_PARTITION_TOKENS,
                         query_start_loc=None, max_query_len=None, causal=True,
                         out=None, workspace=None, work=None, check=False, prefix_packs=None,
-                        decode_plan=None, append=None):
+                        decode_plan=None, append=None, sinks=None):
         """Paged attention of this layer's arena for every row of a step.
 
         Decode (``query_start_loc=None``): one query token per sequence, ``query``
@@ -343,7 +344,22 @@ class PagedKVCache:
         step's newest tokens, key/value ``[S, Hkv, D]`` in the query dtype and int64 slots
         ``[S]`` the caller reserved. The decode quantizes and writes each token into the
         arena and attends to it in the same launch: the outputs and the arena equal
-        ``append(..., reserved=True)`` followed by the call without it."""
+        ``append(..., reserved=True)`` followed by the call without it.
+
+        ``sinks`` (with ``window``, causal, automatic split, no plan or packs): keys
+        ``k < sinks`` stay visible beside the window. Only pages that hold a visible key
+        are read."""
+        if sinks is not None:
+            if type(sinks) is not int or sinks < 1 or window is None:
+                raise ValueError("sinks must be a positive int beside a window")
+            if (prefix_packs is not None or decode_plan is not None or append is not None
+                    or partition_tokens != 0 or not causal):
+                raise ValueError("windows with sinks are causal and take no decode plan, prefix "
+                                 "packs or partition size")
+            return self._bounded_attention(
+                layer, query, block_tables, context_lens, max_context_len=max_context_len,
+                scale=scale, window=window, sinks=sinks, query_start_loc=query_start_loc,
+                max_query_len=max_query_len, out=out, workspace=workspace, work=work, check=check)
         if query.ndim != 3 or query.shape[-1] != self.head_dim or query.device != self.device:
             raise ValueError("query must be [tokens, num_q_heads, head_dim] on the cache device")
         if query.dtype not in _DTYPE_CODES:
@@ -480,6 +496,174 @@ class PagedKVCache:
             self.raise_errors()
         return out
 
+    def paged_attention_weights(self, layer, query, block_tables, context_lens, key_weights, *,
+                                max_context_len, scale=None, query_start_loc=None,
+                                max_query_len=None, out=None, workspace=None, work=None,
+                                check=False):
+        """:meth:`paged_attention` (causal, without a window) that also adds to every key's
+        weight its softmax weight, summed over the call's queries that see it and the heads
+        of its KV head's group. ``key_weights``: the batch's rows of a
+        :class:`~aster_amd.KeyWeights` (``KeyWeights.select``), one per sequence. The
+        weights of the call's own tokens (the last ``n`` keys of a sequence with ``n``
+        queries) start at 0, whatever the row held there; weights behind a sequence's length
+        are left as they are. A call that flags an error may have added its finite rows."""
+        num_seqs = block_tables.shape[0] if isinstance(block_tables, torch.Tensor) else 0
+        require_rows(self, key_weights, num_seqs)
+        if max_context_len > key_weights.weights.capacity:
+            raise ValueError("max_context_len exceeds the key weights' capacity")
+        return self._bounded_attention(
+            layer, query, block_tables, context_lens, max_context_len=max_context_len, scale=scale,
+            query_start_loc=query_start_loc, max_query_len=max_query_len, out=out,
+            workspace=workspace, work=work, check=check, key_weights=key_weights)
+
+    def bounded_workspace_bytes(self, num_seqs, num_q_heads, max_context_len, dtype, *, window=None,
+                                sinks=None, key_weights=False, num_query_tokens=0, max_query_len=0):
+        """Workspace of a call with ``sinks``, or of :meth:`paged_attention_weights`
+        (``key_weights=True``); the last two arguments as the call's packed queries."""
+        return int(_native.lib().astr_paged_attention_i8_bounded_workspace_bytes(
+            num_seqs, num_q_heads, self.num_kv_heads, self.head_dim, _DTYPE_CODES[dtype],
+            num_query_tokens, max_query_len, max_context_len, window or 0, sinks or 0,
+            1 if key_weights else 0))
+
+    def _bounded_attention(self, layer, query, block_tables, context_lens, *, max_context_len,
+                           scale=None, window=None, sinks=None, query_start_loc=None,
+                           max_query_len=None, out=None, workspace=None, work=None, check=False,
+                           key_weights=None):
+        if query.ndim != 3 or query.shape[-1] != self.head_dim or query.device != self.device:
+            raise ValueError("query must be [tokens, num_q_heads, head_dim] on the cache device")
+        if query.dtype not in _DTYPE_CODES:
+            raise UnsupportedAttentionBackend(f"query dtype {query.dtype} is not fp32/fp16/bf16")
+        if query.stride(-1) != 1:
+            raise ValueError("query rows must be contiguous")
+        num_tokens, num_q_heads = query.shape[0], query.shape[1]
+        if num_q_heads % self.num_kv_heads:
+            raise ValueError("Query heads must divide into KV groups")
+        _check_index(block_tables, "block_tables", 2, self.device)
+        _check_index(context_lens, "context_lens", 1, self.device)
+        num_seqs = block_tables.shape[0]
+        if context_lens.shape[0] != num_seqs:
+            raise ValueError("block_tables/context_lens must have one row per sequence")
+        if query_start_loc is None:
+            if num_tokens != num_seqs:
+                raise ValueError("decode attention takes one query row per sequence")
+            max_query_len = 0
+        else:
+            _check_index(query_start_loc, "query_start_loc", 1, self.device)
+            if query_start_loc.shape[0] != num_seqs + 1:
+                raise ValueError("query_start_loc must have num_seqs + 1 entries")
+            if max_query_len is None:
+                lens = query_start_loc[1:] - query_start_loc[:-1]
+                max_query_len = int(lens.max().item()) if num_seqs else 0
+            if type(max_query_len) is not int or max_query_len < 0:
+                raise ValueError("max_query_len must be a non-negative int")
+        if max_context_len > block_tables.shape[1] * self.block_size:
+            raise ValueError("max_context_len exceeds the block table capacity")
+        scale = self.head_dim ** -0.5 if scale is None else float(scale)
+        if not math.isfinite(scale) or scale <= 0:
+            raise ValueError("Attention scale must be finite and positive")
+        if window is not None and (type(window) is not int or window < 1):
+            raise ValueError("Invalid causal/window semantics")
+        if out is None:
+            out = torch.empty_like(query)
+        elif (not isinstance(out, torch.Tensor) or out.shape != query.shape
+              or out.dtype != query.dtype or out.device != self.device or out.stride(-1) != 1):
+            raise ValueError("out must match the query's shape, dtype and device, with "
+                             "contiguous rows")
+        packed = query_start_loc is not None
+        need = self.bounded_workspace_bytes(
+            num_seqs, num_q_heads, max_context_len, query.dtype, window=window, sinks=sinks,
+            key_weights=key_weights is not None, num_query_tokens=num_tokens if packed else 0,
+            max_query_len=max_query_len)
+        if need and workspace is None:
+            workspace = self._scratch(need)
+        elif need:
+            if (not isinstance(workspace, torch.Tensor) or workspace.dtype != torch.uint8
+                    or workspace.device != self.device or not workspace.is_contiguous()):
+                raise ValueError("workspace must be a contiguous uint8 tensor on the cache device")
+            if workspace.numel() < need:
+                raise ValueError(f"workspace of {need} bytes required")
+        stream = torch.cuda.current_stream(self.device).cuda_stream
+        lib = _native.lib()
+        args = [self._descs[layer], query.data_ptr(), _DTYPE_CODES[query.dtype], query.stride(0),
+                query.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
+                query_start_loc.data_ptr() if packed else None, num_tokens if packed else 0,
+                max_query_len, block_tables.data_ptr(), _row_stride(block_tables),
+                context_lens.data_ptr(), num_seqs, num_q_heads, max_context_len, scale]
+        tail = [workspace.data_ptr() if need else None, need, self.err_flag.data_ptr(), stream]
+        with torch.cuda.device(self.device):
+            if key_weights is None:
+                rc = lib.astr_paged_attention_i8_sinks(*args, window, sinks, *tail)
+            else:
+                desc = key_weights.weights.desc(key_weights, layer)
+                rc = lib.astr_paged_attention_i8_key_weights(*args, ctypes.byref(desc), *tail)
+        _native.check(rc, "paged_attention")
+        if work is not None:
+            prefill = packed and max_query_len > 1
+            work.backend, work.fallback_reason = BACKEND, None
+            work.page_launches += (2 if need else 1) + (1 if prefill else 0) + (
+                2 if prefill and key_weights is not None else 0)
+            work.query_tiles += 1
+            work.max_query_tile = max(work.max_query_tile, max_query_len if prefill else 1)
+            work.max_key_tile = max(work.max_key_tile, self.block_size)
+            work.compiler_version = lib.astr_version().decode()
+        if check:
+            self.raise_errors()
+        return out
+
+    def evict(self, block_tables, context_lens, key_weights, *, keep, max_context_len, recent=0,
+              sinks=0, dst_tables=None, into=None, check=False):
+        """Evict all but ``keep`` tokens of every sequence, in every layer and KV head apart:
+        the first ``sinks`` and the last ``recent`` real tokens stay and, of the others, those
+        that gathered the most weight (``key_weights`` as for
+        :meth:`paged_attention_weights`; equal weights: lowest position first). Padding
+        tokens leave, and a sequence of no more real tokens keeps them all. What stays moves,
+        in order, to the first slots: codes, scales and weights, of all layers.
+
+        Without ``dst_tables`` the tokens move within ``block_tables``' pages, which must not
+        be in two rows; with it (int32 ``[S, >= keep / 16]``) into its pages, none of which
+        any row of ``block_tables`` holds, each named once. ``into``: rows of the same
+        :class:`~aster_amd.KeyWeights` that the weights move to (their own rows without).
+        Returns :class:`~aster_amd.EvictedTokens`."""
+        _check_index(block_tables, "block_tables", 2, self.device)
+        _check_index(context_lens, "context_lens", 1, self.device)
+        num_seqs = block_tables.shape[0]
+        if context_lens.shape[0] != num_seqs:
+            raise ValueError("block_tables/context_lens must have one row per sequence")
+        weights = require_rows(self, key_weights, num_seqs)
+        if any(type(v) is not int or v < 0 for v in (keep, recent, sinks)) or keep < 1                 or sinks + recent > keep:
+            raise ValueError("keep must be a positive int that holds the sinks and recent tokens")
+        if max_context_len > block_tables.shape[1] * self.block_size:
+            raise ValueError("max_context_len exceeds the block table capacity")
+        if max_context_len > weights.capacity:
+            raise ValueError("max_context_len exceeds the key weights' capacity")
+        if dst_tables is not None:
+            _check_index(dst_tables, "dst_tables", 2, self.device)
+            if dst_tables.shape[0] != num_seqs or                     dst_tables.shape[1] * self.block_size < min(keep, max_context_len):
+                raise ValueError("dst_tables must hold the tokens that stay, one row per sequence")
+        if into is not None:
+            weights.check(self, into, num_seqs, "into")
+            theirs = {row: i for i, row in enumerate(key_weights.rows)}
+            if any(theirs.get(row, i) != i for i, row in enumerate(into.rows)):
+                raise ValueError("into names another sequence's key weight row")
+        kept = torch.empty((num_seqs, self.num_layers, self.num_kv_heads, keep), dtype=torch.int32,
+                           device=self.device)
+        lengths = torch.empty((num_seqs,), dtype=torch.int32, device=self.device)
+        desc = weights.desc(key_weights)
+        stream = torch.cuda.current_stream(self.device).cuda_stream
+        with torch.cuda.device(self.device):
+            rc = _native.lib().astr_kv_evict(
+                self._descs[0], self.num_layers, self.codes.stride(1), self.scales.stride(1),
+                ctypes.byref(desc), weights.values.stride(1),
+                into.table.data_ptr() if into is not None else None, block_tables.data_ptr(),
+                _row_stride(block_tables), dst_tables.data_ptr() if dst_tables is not None else None,
+                _row_stride(dst_tables) if dst_tables is not None else 0, context_lens.data_ptr(),
+                num_seqs, max_context_len, keep, sinks, recent, kept.data_ptr(),
+                lengths.data_ptr(), self.err_flag.data_ptr(), stream)
+        _native.check(rc, "evict")
+        if check:
+            self.raise_errors()
+        return EvictedTokens(kept, lengths)
+
     def decode_appends(self, dtype):
         """Whether a planned decode of this arena appends the step's ``dtype`` rows itself
         (``paged_attention(append=...)``): bf16/fp16 at head dims 128 and 256 (at 64 the
@@ -545,3 +729,8 @@ def _check_index(tensor, name, ndim, device):
             or tensor.device != device or tensor.stride(-1) != 1):
         raise ValueError(f"{name} must be an int32 device tensor of rank {ndim} with "
                          "contiguous rows")
+
+
+def _row_stride(table):
+    """A table's row stride; a single row's own stride may be anything."""
+    return table.stride(0) if table.shape[0] > 1 else table.shape[1]

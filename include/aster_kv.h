@@ -457,6 +457,100 @@ int astr_paged_attention_i8_planned_append(
     int32_t* err_flag, void* stream);
 
 /*
+ * astr_paged_attention_i8 and, with query_start_loc, astr_paged_attention_varlen_i8 (causal)
+ * in which the first `sinks` keys of every sequence stay visible beside the sliding window:
+ * a query at position p sees key k iff k <= p and (k > p - window or k < sinks). window and
+ * sinks >= 1; no reference counterpart (its windows have no sinks, online_attention.py:183-184).
+ *   query_start_loc: NULL for one query token per sequence (num_query_tokens and
+ *              max_query_len are then not read), else as astr_paged_attention_varlen_i8.
+ *   max_context_len: a longer row raises ASTR_FLAG_BAD_INDEX and is cut to it.
+ *   workspace: >= astr_paged_attention_i8_bounded_workspace_bytes(..., window, sinks, 0)
+ *              bytes, 256-byte aligned (NULL allowed when that is 0); not shared by calls
+ *              that overlap (two captured graphs replayed side by side need one each).
+ * Only the blocks of a sink or window key are read: table entries between them may hold any
+ * id. Rows of fp32 queries with one token come out within fp32 rounding; chunks multiply
+ * softmax weights rounded to f16, as astr_paged_attention_varlen_i8.
+ */
+int astr_paged_attention_i8_sinks(
+    const astr_paged_kv* cache, const void* query, int32_t q_dtype, int64_t q_token_stride,
+    int64_t q_head_stride, void* out, int64_t out_token_stride, int64_t out_head_stride,
+    const int32_t* query_start_loc, int32_t num_query_tokens, int32_t max_query_len,
+    const int32_t* block_tables, int32_t block_table_stride, const int32_t* context_lens,
+    int32_t num_seqs, int32_t num_q_heads, int32_t max_context_len, float scale, int32_t window,
+    int32_t sinks, void* workspace, size_t workspace_bytes, int32_t* err_flag, void* stream);
+
+/*
+ * Weights gathered per key and KV head of one layer (device memory, caller-owned): key t of
+ * sequence s and KV head h at values[rows[s] * row_stride + h * head_stride + t] (row s
+ * itself where rows is NULL). Rows of one call must be distinct: two sequences on one row
+ * race. A row number outside [0, num_rows) raises ASTR_FLAG_BAD_INDEX and that sequence
+ * gathers nothing.
+ */
+typedef struct astr_key_weights {
+  float* values;       /* 16-byte aligned; strides multiples of 4 */
+  int64_t row_stride;  /* floats */
+  int64_t head_stride; /* floats */
+  const int32_t* rows; /* [num_seqs] or NULL */
+  int32_t num_rows;
+  int32_t capacity;    /* tokens of a row, >= max_context_len */
+} astr_key_weights;
+
+/*
+ * Attention without a window (as astr_paged_attention_i8_sinks otherwise: one token per
+ * sequence, or chunks, causal) that adds to each key's weight its softmax weight summed over
+ * the call's queries that see it and the heads of its KV head's group,
+ *   A[k] += sum_{queries p >= k} sum_g softmax(scale q_pg . K)[k],
+ * in fp32 and in a fixed order. Keys of the call's own tokens (the last n of a row of n
+ * queries) start at 0, whatever their place held; keys behind the row's length and padding
+ * keys' sums are left as they are. A query whose scores are not finite raises
+ * ASTR_FLAG_NONFINITE_SCORE and adds nothing. No reference counterpart.
+ *   workspace: >= astr_paged_attention_i8_bounded_workspace_bytes(..., 0, 0, 1) bytes.
+ */
+int astr_paged_attention_i8_key_weights(
+    const astr_paged_kv* cache, const void* query, int32_t q_dtype, int64_t q_token_stride,
+    int64_t q_head_stride, void* out, int64_t out_token_stride, int64_t out_head_stride,
+    const int32_t* query_start_loc, int32_t num_query_tokens, int32_t max_query_len,
+    const int32_t* block_tables, int32_t block_table_stride, const int32_t* context_lens,
+    int32_t num_seqs, int32_t num_q_heads, int32_t max_context_len, float scale,
+    const astr_key_weights* weights, void* workspace, size_t workspace_bytes, int32_t* err_flag,
+    void* stream);
+
+/* Workspace bytes of astr_paged_attention_i8_sinks and astr_paged_attention_i8_key_weights
+ * (key_weights != 0). num_query_tokens and max_query_len: 0 without query_start_loc. */
+size_t astr_paged_attention_i8_bounded_workspace_bytes(
+    int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+    int32_t q_dtype, int32_t num_query_tokens, int32_t max_query_len, int32_t max_context_len,
+    int32_t window, int32_t sinks, int32_t key_weights);
+
+/*
+ * Eviction by gathered weight: of each sequence's real tokens (key_valid; padding leaves) the
+ * first `sinks` and the last `recent` stay, and of the others the heaviest per layer and KV
+ * head, `keep` in all (all of them where there are no more), equal weights lowest index
+ * first, NaN weights last. They move to the front in their order: codes and scales of every
+ * layer, weights, and (where the arena has them) key_valid bytes, which become 1. No
+ * reference counterpart.
+ *   cache, weights: of layer 0; code_layer_stride (bytes), scale_layer_stride and
+ *              weight_layer_stride (floats) lead to the next layer's.
+ *   dst_block_tables: NULL moves within block_tables' pages, which must then belong to
+ *              their sequence alone (a page in two rows races); else [num_seqs,
+ *              dst_block_table_stride] pages that no row of block_tables holds, each once.
+ *   dst_weight_rows: NULL compacts the weights within their rows; else the rows they move to,
+ *              none of them a row of another sequence.
+ *   kept: int32 [num_seqs, num_layers, num_kv_heads, keep], the tokens that stay (-1 behind
+ *              the last); new_lens: int32 [num_seqs], their number.
+ * Slots behind new_lens keep what they hold. A length or id out of range raises
+ * ASTR_FLAG_BAD_INDEX: the row is cut, the token does not move.
+ */
+int astr_kv_evict(const astr_paged_kv* cache, int32_t num_layers, int64_t code_layer_stride,
+                  int64_t scale_layer_stride, const astr_key_weights* weights,
+                  int64_t weight_layer_stride, const int32_t* dst_weight_rows,
+                  const int32_t* block_tables, int32_t block_table_stride,
+                  const int32_t* dst_block_tables, int32_t dst_block_table_stride,
+                  const int32_t* context_lens, int32_t num_seqs, int32_t max_context_len,
+                  int32_t keep, int32_t sinks, int32_t recent, int32_t* kept, int32_t* new_lens,
+                  int32_t* err_flag, void* stream);
+
+/*
  * Bit-exact copy of whole blocks: block i of `num_blocks` goes from
  *   src + (src_index ? src_index[i] : i) * src_stride
  * to
