@@ -43,7 +43,7 @@ struct Shape {
 struct Plan {
   int32_t waves, part_blocks, parts;     // decode
   int64_t score_stride;
-  int32_t chunk_pieces, chunk_steps;     // chunks' weights
+  int32_t chunk_pieces, chunk_steps, column_pieces, column_tiles;  // chunks' weights
   size_t o_bytes, ml_bytes, score_bytes, chunk_bytes, prefill_bytes;
   size_t decode() const { return o_bytes + ml_bytes + score_bytes; }
   // the decode launches, the prefill launch and the chunks' weights follow one another on the
@@ -60,6 +60,8 @@ int64_t visible_blocks(const Shape& s) {
   return std::min(all + 1, seen);  // (a block of sinks and window keys is listed twice)
 }
 
+constexpr int64_t kMostPieces = 32;  // of a chunk's keys or columns
+
 // Partials of the prefill launch's split units: what a call of this shape may use.
 constexpr size_t kPrefillPartials = (size_t)64 << 20;
 
@@ -68,8 +70,12 @@ Plan plan_call(const Shape& s) {
   const int64_t blocks = std::max<int64_t>(visible_blocks(s), 1);
   const int64_t units = std::max<int64_t>((int64_t)s.num_seqs * s.num_kv_heads, 1);
   const int64_t cus = device_cus();
-  const int wide = wide_waves(s.head_dim);
-  p.waves = units <= cus ? wide : 4;
+  // A workgroup of 16 waves (8 at head dim 256, where the LDS holds no more stages) has the
+  // CU to itself, two of 8 share it and hide each other's first loads and last merge: 16 where
+  // every CU takes several units (128 rows, window 4096: 164 us a call against 167 with 8 waves and
+  // 174 with 4), 8 where it takes one or none (48 rows, 4 KV heads, window 1024: 15.3 against
+  // 17.8 and 20.2).
+  p.waves = units <= cus ? 8 : wide_waves(s.head_dim);
   // pieces: of 64 blocks a wave at most, and enough of them to give every CU 16 waves
   int64_t parts = (blocks + (int64_t)p.waves * kIdsPerWave - 1) / ((int64_t)p.waves * kIdsPerWave);
   const int64_t want = 16 * cus / (units * p.waves);
@@ -95,13 +101,26 @@ Plan plan_call(const Shape& s) {
           std::min((int64_t)s.num_seqs * (((int64_t)s.max_q_len * group + 127) / 128),
                    (int64_t)s.num_q_tokens * group / 128 + s.num_seqs) * s.num_kv_heads, 1);
       const int64_t steps = (blocks + kWaves - 1) / kWaves;
-      int64_t pieces = std::min<int64_t>(std::min<int64_t>(2 * cus / ctiles, steps / 8), 32);
-      pieces = std::max<int64_t>(pieces, 1);
-      p.chunk_steps = (int32_t)((steps + pieces - 1) / pieces);
+      // first pass: pieces of steps for eight workgroups a CU, of 8 steps at least (a prompt's
+      // early tokens see few keys, half of these workgroups have nothing to do)
+      int64_t per = std::max<int64_t>((ctiles * steps + 8 * cus - 1) / (8 * cus), 8);
+      per = std::max(per, (steps + kMostPieces - 1) / kMostPieces);
+      p.chunk_steps = (int32_t)std::min(per, steps);
       p.chunk_pieces = (int32_t)((steps + p.chunk_steps - 1) / p.chunk_steps);
+      // second pass: pieces of the column tiles for as many, of 16 tiles at least
+      const int64_t keys = kWaves * (s.head_dim == 256 ? 32 : 64);
+      const int64_t units = (int64_t)s.num_seqs * s.num_kv_heads * ((s.max_context + keys - 1) / keys);
+      const int64_t columns = ((int64_t)s.max_q_len * group + 31) / 32;
+      int64_t pieces = std::min<int64_t>(8 * cus / std::max<int64_t>(units, 1), columns / 16);
+      pieces = std::max<int64_t>(std::min<int64_t>(pieces, kMostPieces), 1);
+      p.column_tiles = (int32_t)((columns + pieces - 1) / pieces);
+      p.column_pieces = (int32_t)((columns + p.column_tiles - 1) / p.column_tiles);
       const size_t tiles = ((size_t)s.num_q_tokens * group / 32 + s.num_seqs) * s.num_kv_heads;
       p.chunk_bytes = align256(tiles * (32 * 8 * (size_t)(1 + p.chunk_pieces) +
                                         (size_t)s.terms * s.head_dim * 64));
+      if (p.column_pieces > 1)
+        p.chunk_bytes += align256((size_t)s.num_seqs * s.num_kv_heads * p.column_pieces *
+                                  p.score_stride * sizeof(float));
     }
   }
   return p;
@@ -249,9 +268,8 @@ int bounded_attention(const Call& c) {
   hipStream_t s = static_cast<hipStream_t>(c.stream);
   const bool chunks = packed && c.max_query_len >= 2;
   // Where every row must carry max_query_len tokens no decode row is left (an offset array that
-  // says otherwise is served all the same, by the chunk kernels; key weights refuse it: rows of
-  // one token need the decode kernel there).
-  const bool only_chunks = chunks && w == nullptr && c.q_dtype != ASTR_F32 &&
+  // says otherwise is served all the same, by the chunk kernels).
+  const bool only_chunks = chunks && c.q_dtype != ASTR_F32 &&
                            !(cache->head_dim == 256 && group == 16) &&
                            (int64_t)c.num_seqs * c.max_query_len == c.num_query_tokens;
   if (!only_chunks) {
@@ -266,9 +284,12 @@ int bounded_attention(const Call& c) {
   const int rc = w == nullptr && c.sinks > 0 ? launch_prefill_sinks(chunk, c.q_dtype, s)
                                              : launch_prefill(chunk, c.q_dtype, s);
   if (rc != 0 || w == nullptr) return rc;
-  a.chunk_ml = static_cast<float*>(c.workspace);
+  a.chunk_ws = static_cast<float*>(c.workspace);
+  a.min_rows = chunk.pf_min_rows;
   a.chunk_pieces = plan.chunk_pieces;
   a.chunk_steps = plan.chunk_steps;
+  a.column_pieces = plan.column_pieces;
+  a.column_tiles = plan.column_tiles;
   return launch_chunk_weights(a, c.q_dtype, s);
 }
 

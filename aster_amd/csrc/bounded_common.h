@@ -26,10 +26,12 @@ struct BoundedArgs : AttnArgs {
   // base-2 scores of every key, [num_seqs * num_kv_heads * group][score_stride]; weights only
   float* scores;
   int64_t score_stride;
-  // chunks (key weights): (m, l) of every (query token, head) and piece of its keys,
-  // [piece][num_q_tokens][num_q_heads], and the pieces' key steps of 64
-  float* chunk_ml;
+  // chunks (key weights, chunk_weights.hip): their workspace; the first pass's pieces of the keys
+  // and their steps of 64 keys; the second's pieces of the column tiles and their length
+  float* chunk_ws;
+  int32_t min_rows;  // fewest queries of a row the chunk kernels take
   int32_t chunk_pieces, chunk_steps;
+  int32_t column_pieces, column_tiles;
 };
 
 // What sequence `seq` sees: keys [0, sinks) in blocks [0, sink_blocks) and keys [kv_begin,

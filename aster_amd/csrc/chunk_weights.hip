@@ -6,7 +6,7 @@
 // Two passes over the scores, which are formed twice (2 D operations each, cheaper than 4
 // bytes written and read per score): the first keeps 32 (token, head) columns per wave and
 // streams the keys (64 per step, converted once to f16 operands in LDS for the workgroup's
-// 128 columns) under a running maximum and sum; the second keeps KT keys per wave and streams
+// 128 columns) under a running maximum and sum; the second keeps 64 keys per wave and streams
 // the columns, whose f16 operands, factor and lse the first left in the workspace in the
 // order the second's lanes read them. In both, v_mfma_f32_32x32x16_f16 gives lane (c, h) the
 // scores of column c and keys 8 x + 4 h + y (element 4 x + y), so that the first pass reduces
@@ -15,7 +15,7 @@
 //
 // Scores: K codes exact in f16 against one f16 term of a 16-bit query (exact, scaled by a
 // power of two per column) or two of an fp32 one (22 bits), fp32 accumulation.
-#include <type_traits>
+#include <climits>
 
 #include "bounded_common.h"
 
@@ -52,19 +52,26 @@ struct ColumnPlace {
   }
 };
 
-// The workspace: per column {factor, lse}, per piece and column {m, l}, the operands.
+// The workspace: per column {factor, lse}, per piece and column {m, l}, the operands, and the
+// column pieces' sums, one row of score_stride keys per (sequence, KV head) and piece.
 struct ChunkWs {
   float2_t* cols;
   float2_t* ml;
   half8_t* ops;
+  float* sums;
   int64_t columns;
-  __host__ __device__ explicit ChunkWs(const BoundedArgs& a) {
+  __host__ __device__ ChunkWs(const BoundedArgs& a, int op_halves) {
     columns = ColumnPlace::tiles(a) * a.cache.num_kv_heads * 32;
-    cols = reinterpret_cast<float2_t*>(a.chunk_ml);
+    cols = reinterpret_cast<float2_t*>(a.chunk_ws);
     ml = cols + columns;
     ops = reinterpret_cast<half8_t*>(ml + a.chunk_pieces * columns);
+    sums = reinterpret_cast<float*>(ops + columns * (op_halves / 8));
   }
 };
+template <typename QT, int D>
+__host__ __device__ ChunkWs chunk_ws(const BoundedArgs& a) {
+  return ChunkWs(a, ColumnOp<QT, D>::kTerms * D);
+}
 
 struct ChunkRow {
   int q0, n, ctx, pos0;
@@ -75,13 +82,23 @@ __device__ __forceinline__ ChunkRow chunk_row(const BoundedArgs& a, int seq) {
   ChunkRow r;
   r.n = seq_queries(a, seq, r.q0);
   r.ctx = bounded_ctx(a, a.context_lens[seq], false);
-  if (r.n < 2 || r.ctx < r.n) r.n = 0;
+  if (r.n < a.min_rows || r.ctx < r.n) r.n = 0;
   r.pos0 = r.ctx - r.n;
   return r;
 }
 
 __device__ __forceinline__ float log_sum(float m, float l) {
   return l > 0.f ? m + __builtin_amdgcn_logf(l) : INFINITY;
+}
+
+// The workgroup's piece and tile. Workgroups are dealt to the 8 XCDs in turn, and under the causal
+// mask a piece's or a tile's number says how much of it there is: pieces side by side left some
+// XCDs little to do (2000 tokens, first pass: 67 us, 51 with them apart), and so does a number
+// of tiles that 8 divides, against which each piece's tiles begin one later.
+__device__ __forceinline__ void unit_of(int pieces, int& piece, int& tile) {
+  const int tiles = gridDim.x / pieces;
+  piece = blockIdx.x / tiles;
+  tile = (blockIdx.x % tiles + piece) % tiles;
 }
 
 template <int D>
@@ -95,7 +112,10 @@ template <typename QT, int D>
 __global__ __launch_bounds__(256, 2) void chunk_stats_kernel(BoundedArgs a) {
   using Op = ColumnOp<QT, D>;
   __shared__ StatsLds<D> L;
-  const int piece = blockIdx.x % a.chunk_pieces, ctile = blockIdx.x / a.chunk_pieces;
+  // the latest tokens, which see the most keys, first
+  int piece, ctile;
+  unit_of(a.chunk_pieces, piece, ctile);
+  ctile = (int)(gridDim.x / a.chunk_pieces) - 1 - ctile;
   const int kvh = blockIdx.y, seq = blockIdx.z;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave;
@@ -103,58 +123,92 @@ __global__ __launch_bounds__(256, 2) void chunk_stats_kernel(BoundedArgs a) {
   const ChunkRow row = chunk_row(a, seq);
   const int f0 = ctile * 128;
   if (f0 >= row.n * G) return;
+  const int gs = __builtin_ctz(G);  // (a power of two)
   // the keys that the workgroup's last column sees, its piece of them
-  const int last_tok = min(row.n - 1, (f0 + 127) / G);
+  const int last_tok = min(row.n - 1, (f0 + 127) >> gs);
   const int blocks = (row.pos0 + last_tok) / kBlockTokens + 1;
   const int b0 = piece * a.chunk_steps * kWaves;
   const int b1 = min(blocks, b0 + a.chunk_steps * kWaves);
   const int nsteps = b1 > b0 ? (b1 - b0 + kWaves - 1) / kWaves : 0;
 
-  // ---- the wave's columns
-  const int f = f0 + wave * 32 + (lane & 31), h = lane >> 5;
+  const ChunkWs ws = chunk_ws<QT, D>(a);
+  const int64_t tile = ColumnPlace(a, seq, kvh, row.q0).tile0 + ctile * 4 + wave;
+  const bool used = f0 + wave * 32 < row.n * G;  // the wave's tile has a place
+  if (nsteps == 0 && piece > 0) {  // past the keys that the workgroup's columns see
+    if (used && lane < 32) ws.ml[piece * ws.columns + tile * 32 + lane] = float2_t{-FLT_MAX, 0.f};
+    return;
+  }
+
+  // ---- the wave's columns: rows read whole (lane `part` of D / 8 takes eight elements), their
+  // f16 terms through LDS into the operand's order, and into the workspace. (Read by operand
+  // lanes, 16 bytes of 64 rows at a time, the rows of a CU's 16 waves did not stay in its cache:
+  // 15 us before the first step of a 2000-token prompt.)
+  const int h = lane >> 5;
+  const int f = f0 + wave * 32 + (lane & 31);
   const bool valid = f < row.n * G;
-  const int tok = valid ? f / G : last_tok, head = kvh * G + (valid ? f % G : 0);
-  const int pos = row.pos0 + tok;
+  const int pos = row.pos0 + (valid ? f >> gs : last_tok);
   Op q;
   float factor;
   {
-    const QT* qp = static_cast<const QT*>(a.q) + (int64_t)(row.q0 + tok) * a.q_tok +
-                   (int64_t)head * a.q_head + 8 * h;
-    float x[D / 16][8];
-    float mx = 0.f;
+    constexpr int kLanes = D / 8, kRows = kWave / kLanes, kLoads = 32 / kRows;
+    static_assert(kWaves * Op::kChunks * kWave * 16 <= sizeof(L.k), "a term's operands fit the buffers");
+    static_assert(kWaves * 32 * sizeof(float) <= sizeof(L.ks), "the factors fit theirs");
+    struct alignas(8 * sizeof(QT) > 16 ? 16 : 8 * sizeof(QT)) Run {
+      QT e[8];
+    };
+    const int part = lane % kLanes, sub = lane / kLanes;
+    half8_t* const terms = reinterpret_cast<half8_t*>(L.k) + wave * Op::kChunks * kWave;
+    float* const factors = reinterpret_cast<float*>(L.ks) + wave * 32;
+    constexpr int kBatch = kLoads < 8 ? kLoads : 8;  // rows on their way together
 #pragma unroll
-    for (int cc = 0; cc < D / 16; ++cc) {
-      struct alignas(16) Run {
-        QT e[8];
-      };
-      const Run run = *reinterpret_cast<const Run*>(qp + 16 * cc);
+    for (int t = 0; t < Op::kTerms; ++t) {  // (fp32 queries read their rows for each term)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[cc][i] = valid ? to_float<QT>(run.e[i]) : 0.f;
-        mx = vmax(mx, fabsf(x[cc][i]));  // NaN-propagating
+      for (int i0 = 0; i0 < kLoads; i0 += kBatch) {
+        Run run[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const int fi = min(f0 + wave * 32 + (i0 + i) * kRows + sub, row.n * G - 1);
+          run[i] = *reinterpret_cast<const Run*>(static_cast<const QT*>(a.q) +
+                                                 (int64_t)(row.q0 + (fi >> gs)) * a.q_tok +
+                                                 (int64_t)(kvh * G + (fi & (G - 1))) * a.q_head + 8 * part);
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const int c = (i0 + i) * kRows + sub;
+          float x[8], mx = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            x[e] = to_float<QT>(run[i].e[e]);
+            mx = vmax(mx, fabsf(x[e]));  // NaN-propagating
+          }
+#pragma unroll
+          for (int b = 1; b < kLanes; b <<= 1) mx = vmax(mx, shfl_xor(mx, b));
+          // a column that is not finite enters as zeros, of no weight: its lse comes out infinite
+          const bool finite = __builtin_isfinite(mx);
+          int ex = 15;
+          if (finite && mx > 0.f) frexpf(mx, &ex);
+          ex = max(ex - 15, -126);
+          const float down = finite && f0 + wave * 32 + c < row.n * G ? ldexpf(1.f, -ex) : 0.f;
+          half8_t term;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            float v = down == 0.f ? 0.f : x[e] * down;  // exact
+            if constexpr (Op::kTerms == 2) asm volatile("" : "+v"(v));  // one value for both terms
+            const _Float16 hi = (_Float16)v;
+            term[e] = t == 0 ? hi : (_Float16)(v - (float)hi);
+          }
+          terms[(part / 2) * kWave + 32 * (part % 2) + c] = term;
+          if (part == 0)
+            factors[c] = finite ? ldexpf(1.f, ex) * a.qk_scale_log2 * code_scale<KF>() : __builtin_nanf("");
+        }
       }
+      __builtin_amdgcn_wave_barrier();  // a wave's LDS accesses complete in order
+#pragma unroll
+      for (int cc = 0; cc < Op::kChunks; ++cc) q.op[t][cc] = terms[cc * kWave + lane];
+      factor = valid ? factors[lane & 31] : 0.f;
+      __builtin_amdgcn_wave_barrier();
     }
-    mx = vmax(mx, shfl_xor(mx, 32));
-    // a column that is not finite enters as zeros, of no weight: its lse comes out infinite
-    const bool finite = __builtin_isfinite(mx);
-    int ex = 15;
-    if (finite && mx > 0.f) frexpf(mx, &ex);
-    ex = max(ex - 15, -126);
-#pragma unroll
-    for (int cc = 0; cc < D / 16; ++cc)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float v = finite ? ldexpf(x[cc][i], -ex) : 0.f;
-        const _Float16 hi = (_Float16)v;
-        q.op[0][cc][i] = hi;
-        if constexpr (Op::kTerms == 2) q.op[1][cc][i] = (_Float16)(v - (float)hi);
-      }
-    factor = finite ? ldexpf(1.f, ex) * a.qk_scale_log2 * code_scale<KF>() : __builtin_nanf("");
-    factor = valid ? factor : 0.f;
   }
-  const ChunkWs ws(a);
-  const int64_t tile = ColumnPlace(a, seq, kvh, row.q0).tile0 + ctile * 4 + wave;
-  const bool used = f0 + wave * 32 < row.n * G;  // the wave's tile has a place
   if (piece == 0 && used) {
 #pragma unroll
     for (int t = 0; t < Op::kTerms; ++t)
@@ -162,6 +216,7 @@ __global__ __launch_bounds__(256, 2) void chunk_stats_kernel(BoundedArgs a) {
       for (int cc = 0; cc < Op::kChunks; ++cc)
         ws.ops[((tile * Op::kTerms + t) * Op::kChunks + cc) * kWave + lane] = q.op[t][cc];
   }
+  __syncthreads();  // the buffers are the keys' from here on
 
   // ---- the keys
   const int32_t* bt = a.block_tables + (int64_t)seq * a.bt_stride;
@@ -208,7 +263,7 @@ __global__ __launch_bounds__(256, 2) void chunk_stats_kernel(BoundedArgs a) {
   }
   __syncthreads();
   // every column of the wave sees the keys below `inner`
-  const int inner = row.pos0 + min(row.n - 1, (f0 + wave * 32) / G) + 1;
+  const int inner = row.pos0 + min(row.n - 1, (f0 + wave * 32) >> gs) + 1;
   for (int i = 0; i < nsteps; ++i) {
     const int buf = i & 1;
 #pragma unroll
@@ -285,7 +340,7 @@ __global__ __launch_bounds__(256, 2) void chunk_stats_kernel(BoundedArgs a) {
 
 // The pieces' states joined (a piece past a column's keys left l = 0).
 __global__ __launch_bounds__(256) void chunk_lse_kernel(BoundedArgs a) {
-  const ChunkWs ws(a);
+  const ChunkWs ws(a, 0);
   const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (at >= ws.columns) return;
   float m = -FLT_MAX;
@@ -298,7 +353,28 @@ __global__ __launch_bounds__(256) void chunk_lse_kernel(BoundedArgs a) {
   ws.cols[at][1] = log_sum(m, l);
 }
 
-// Keys of one workgroup: 64 in two tiles, 32 at head dim 256 (the operands fill the registers).
+// The first column tile with a token that sees key k0.
+__device__ __forceinline__ int column_first(const ChunkRow& row, int k0, int group) {
+  return max(0, k0 - row.pos0) * group / 32;
+}
+
+// Adds what a key gathered.
+__device__ __forceinline__ void add_key(const BoundedArgs& a, const ChunkRow& row, const int32_t* bt,
+                                        int64_t wrow, int kvh, int key, float v) {
+  if (key >= a.kw.capacity) return;
+  if (a.cache.key_valid != nullptr) {
+    const int id = bt[key / kBlockTokens];
+    if ((unsigned)id < (unsigned)a.cache.num_blocks &&
+        a.cache.key_valid[(int64_t)id * kBlockTokens + key % kBlockTokens] == 0)
+      v = 0.f;  // a padding key
+  }
+  v = __builtin_isfinite(v) ? v : 0.f;  // a key whose own scale is not finite
+  float* w = a.kw.values + wrow * a.kw.row_stride + kvh * a.kw.head_stride + key;
+  *w = (key >= row.pos0 ? 0.f : *w) + v;
+}
+
+// Keys of one wave: 64 in two tiles, 32 at head dim 256 (the operands fill the registers). The
+// workgroup's waves take consecutive keys and go through the same columns.
 template <int D>
 constexpr int column_sum_keys() { return D == 256 ? 32 : 64; }
 
@@ -306,19 +382,26 @@ template <typename QT, int D>
 __global__ __launch_bounds__(256, 2) void column_sum_kernel(BoundedArgs a) {
   using Op = ColumnOp<QT, D>;
   constexpr int KT = column_sum_keys<D>(), NT = KT / 32;
-  __shared__ float red[kWaves][KT];
   const int kvh = blockIdx.y, seq = blockIdx.z;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave;
   const int h = lane >> 5;
-  const int G = a.group;
+  const int G = a.group, gs = __builtin_ctz(G);
   const ChunkRow row = chunk_row(a, seq);
-  const int k0 = blockIdx.x * KT;
+  int piece, ktile;
+  unit_of(a.column_pieces, piece, ktile);
+  piece = a.column_pieces - 1 - piece;  // (every key is seen by the last)
+  const int k0 = (ktile * kWaves + wave) * KT;
   if (row.n == 0 || k0 >= row.ctx) return;
+  // the column tiles from the first token that sees key k0 on, the workgroup's piece of them
+  const int first = max(column_first(row, k0, G), piece * a.column_tiles);
+  const int tiles = min((row.n * G + 31) / 32,
+                        piece == a.column_pieces - 1 ? INT_MAX : (piece + 1) * a.column_tiles);
+  if (first >= tiles) return;
   const int64_t wrow = weight_row(a, seq, false);
   if (wrow < 0) return;
 
-  // ---- the workgroup's keys, as operands in every wave's registers: lane (key, h)
+  // ---- the wave's keys, as operands in its registers: lane (key, h)
   const int32_t* bt = a.block_tables + (int64_t)seq * a.bt_stride;
   const int last_blk = (row.ctx - 1) / kBlockTokens;
   half8_t kop[NT][Op::kChunks];
@@ -350,76 +433,100 @@ __global__ __launch_bounds__(256, 2) void column_sum_kernel(BoundedArgs a) {
     }
   }
 
-  // ---- the column tiles from the first token that sees key k0 on, dealt to the waves
-  const ChunkWs ws(a);
+  // ---- the columns
+  const ChunkWs ws = chunk_ws<QT, D>(a);
   const int64_t tile0 = ColumnPlace(a, seq, kvh, row.q0).tile0;
-  const int tiles = (row.n * G + 31) / 32;
-  const int first = max(0, k0 - row.pos0) * G / 32;
   float sum[NT][16];
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int j = 0; j < 16; ++j) sum[t][j] = 0.f;
-  Op q;
+  half8_t q[Op::kChunks];  // (a second term is read when the first has been used)
   float2_t col = {0.f, INFINITY};
+  auto load_term = [&](int c, int t) __attribute__((always_inline)) {
+#pragma unroll
+    for (int cc = 0; cc < Op::kChunks; ++cc)
+      q[cc] = ws.ops[(((tile0 + c) * Op::kTerms + t) * Op::kChunks + cc) * kWave + lane];
+  };
   auto load = [&](int c) __attribute__((always_inline)) {
-#pragma unroll
-    for (int t = 0; t < Op::kTerms; ++t)
-#pragma unroll
-      for (int cc = 0; cc < Op::kChunks; ++cc)
-        q.op[t][cc] = ws.ops[(((tile0 + c) * Op::kTerms + t) * Op::kChunks + cc) * kWave + lane];
+    load_term(c, 0);
     col = ws.cols[(tile0 + c) * 32 + (lane & 31)];
   };
-  if (first + wave < tiles) load(first + wave);
-  for (int c = first + wave; c < tiles; c += kWaves) {
+  load(first);
+  for (int c = first; c < tiles; ++c) {
     float16v_t s[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) s[t][j] = 0.f;
-#pragma unroll
-      for (int x = 0; x < Op::kTerms; ++x)
-#pragma unroll
-        for (int cc = 0; cc < Op::kChunks; ++cc)
-          s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kop[t][cc], q.op[x][cc], s[t], 0, 0, 0);
-    }
-    const float factor = col[0], lse = col[1];
-    const int pos = row.pos0 + min(row.n - 1, (c * 32 + (lane & 31)) / G);
-    const bool edge = row.pos0 + c * 32 / G < k0 + KT - 1;  // some column does not see some key
-    if (c + kWaves < tiles) load(c + kWaves);
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j] * ks[t][j / 4][j % 4], factor, -lse));
-        if (edge) p = k0 + 32 * t + 8 * (j / 4) + 4 * h + j % 4 <= pos ? p : 0.f;
-        sum[t][j] += p;
-      }
+      for (int j = 0; j < 16; ++j) s[t][j] = 0.f;
+#pragma unroll
+    for (int x = 0; x < Op::kTerms; ++x) {
+      if (x > 0) load_term(c, x);
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int cc = 0; cc < Op::kChunks; ++cc)
+          s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kop[t][cc], q[cc], s[t], 0, 0, 0);
+    }
+    const float factor = col[0], lse = col[1];
+    const int pos = row.pos0 + min(row.n - 1, (c * 32 + (lane & 31)) >> gs);
+    if (c + 1 < tiles) load(c + 1);
+    if (row.pos0 + (c * 32 >> gs) < k0 + KT - 1) {  // some column does not see some key
+      asm volatile("");  // keeps this a branch: if-converted, the other tiles would pay for it
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int32_t before = pos - (k0 + 32 * t + 8 * (j / 4) + 4 * h + j % 4);  // < 0: not seen
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j] * ks[t][j / 4][j % 4], factor, -lse));
+          sum[t][j] += __builtin_bit_cast(float, __builtin_bit_cast(int32_t, p) & ~(before >> 31));
+        }
+    } else {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          sum[t][j] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j] * ks[t][j / 4][j % 4], factor, -lse));
+    }
   }
+  // ---- over the columns: lane 32 h + 16 t + j keeps the sum of key 32 t + 8 (j / 4) + 4 h + j % 4
+  float v = 0.f;
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
-      float v = group_sum<16>(sum[t][j]);
-      v += shfl_xor(v, 16);
-      if ((lane & 31) == 0) red[wave][32 * t + 8 * (j / 4) + 4 * h + j % 4] = v;
+      float x = group_sum<16>(sum[t][j]);
+      x += shfl_xor(x, 16);
+      v = (lane & 31) == 16 * t + j ? x : v;
     }
-  __syncthreads();
-  const int key = k0 + threadIdx.x;
-  if ((int)threadIdx.x < KT && key < row.ctx && key < a.kw.capacity) {
-    float v = red[0][threadIdx.x];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) v += red[w][threadIdx.x];
-    if (a.cache.key_valid != nullptr) {
-      const int id = bt[key / kBlockTokens];
-      if ((unsigned)id < (unsigned)a.cache.num_blocks &&
-          a.cache.key_valid[(int64_t)id * kBlockTokens + key % kBlockTokens] == 0)
-        v = 0.f;  // a padding key
-    }
-    v = __builtin_isfinite(v) ? v : 0.f;  // a key whose own scale is not finite
-    float* w = a.kw.values + wrow * a.kw.row_stride + kvh * a.kw.head_stride + key;
-    *w = (key >= row.pos0 ? 0.f : *w) + v;
+  const int j = lane & 15, t = lane >> 4 & 1;
+  const int key = k0 + 32 * t + 8 * (j / 4) + 4 * h + j % 4;
+  if (t < NT && key < row.ctx) {
+    if (a.column_pieces == 1)
+      add_key(a, row, bt, wrow, kvh, key, v);
+    else
+      ws.sums[(((int64_t)seq * a.cache.num_kv_heads + kvh) * a.column_pieces + piece) * a.score_stride +
+              key] = v;
   }
+}
+
+// The column pieces' sums joined, a key per thread.
+__global__ __launch_bounds__(256) void column_join_kernel(BoundedArgs a, int op_halves, int keys) {
+  const int kvh = blockIdx.y, seq = blockIdx.z;
+  const ChunkRow row = chunk_row(a, seq);
+  const int key = blockIdx.x * 256 + threadIdx.x;
+  if (row.n == 0 || key >= row.ctx) return;
+  const int64_t wrow = weight_row(a, seq, false);
+  if (wrow < 0) return;
+  const float* sums = ChunkWs(a, op_halves).sums +
+                      ((int64_t)seq * a.cache.num_kv_heads + kvh) * a.column_pieces * a.score_stride + key;
+  // the pieces that hold tiles which see the key's tile of keys
+  const int first = column_first(row, key / keys * keys, a.group);
+  const int tiles = (row.n * a.group + 31) / 32;
+  float v = 0.f;
+  for (int p = min(first / a.column_tiles, a.column_pieces - 1); p < a.column_pieces; ++p)
+    if (p * a.column_tiles < tiles) v += sums[p * a.score_stride];
+  add_key(a, row, a.block_tables + (int64_t)seq * a.bt_stride, wrow, kvh, key, v);
 }
 
 template <typename QT, int D>
@@ -430,13 +537,17 @@ int launch(const BoundedArgs& a, hipStream_t stream) {
   hipLaunchKernelGGL((chunk_stats_kernel<QT, D>),
                      dim3((uint32_t)(ctiles * a.chunk_pieces), hkv, seqs), dim3(256), 0, stream, a);
   if (a.chunk_pieces > 1) {
-    const int64_t columns = ChunkWs(a).columns;
+    const int64_t columns = ChunkWs(a, 0).columns;
     hipLaunchKernelGGL(chunk_lse_kernel, dim3((uint32_t)((columns + 255) / 256)), dim3(256), 0,
                        stream, a);
   }
   constexpr int KT = column_sum_keys<D>();
-  hipLaunchKernelGGL((column_sum_kernel<QT, D>), dim3((uint32_t)((a.max_context + KT - 1) / KT), hkv, seqs),
+  const int64_t ktiles = ((int64_t)a.max_context + kWaves * KT - 1) / (kWaves * KT);
+  hipLaunchKernelGGL((column_sum_kernel<QT, D>), dim3((uint32_t)(ktiles * a.column_pieces), hkv, seqs),
                      dim3(256), 0, stream, a);
+  if (a.column_pieces > 1)
+    hipLaunchKernelGGL(column_join_kernel, dim3((uint32_t)((a.max_context + 255) / 256), hkv, seqs),
+                       dim3(256), 0, stream, a, ColumnOp<QT, D>::kTerms * D, KT);
   const hipError_t err = hipGetLastError();
   return err == hipSuccess ? 0 : hip_fail(err, "key weights (chunks) launch");
 }

@@ -33,62 +33,79 @@ constexpr int KF = ASTR_KF;  // this translation unit's code format
 
 constexpr int kTileTokens = 1024;  // keys whose weights one workgroup of the second launch adds
 
-// The FP8 query operand: f16 terms of the query column, scaled by the power of two that
-// brings its largest element into [2^14, 2^15) (then exact for 16-bit queries, whose
-// elements below 2^-28 of that maximum round by 2^-39 of it; 22 bits of fp32 ones).
+// The group's query columns as B operands, built once per workgroup (four elements a lane and
+// wave at a time) and read by every wave: for all of them the arithmetic is 500 instructions,
+// as much as four blocks take, and 16 waves share a CU. Lane (qg, r) holds elements d = 16 qg + 64 h + [0, 16) of head r.
+//   int8 codes: three int8 terms of q * kQRange / max|q| (query_terms: 22 bits of the query)
+//   FP8 codes: f16 terms of the column scaled by the power of two that brings its largest
+//     element into [2^14, 2^15): one of 16-bit queries (exact; below 2^-28 of that maximum to
+//     2^-39 of it), two of fp32 ones (22 bits)
 template <typename QT, int D>
-struct HalfQuery {
-  static constexpr int kTerms = sizeof(QT) == 4 ? 2 : 1;
-  half8_t op[kTerms][D / 32];
+struct SharedQuery {
+  static constexpr int kTerms = KF == kInt8 ? 3 : sizeof(QT) == 4 ? 2 : 1;
+  static constexpr int kPer = KF == kInt8 ? 1 : 2;  // operands of 64 elements of a term
+  static constexpr int kOps = kTerms * kPer * (D / 64);
+  int4_t op[kOps][kWave];
+  float factor[16];  // of the columns' scores; NaN for a column that is not finite
+  __device__ static constexpr int at(int term, int h, int sub) { return (term * (D / 64) + h) * kPer + sub; }
 };
 
-// Builds the lane's query operand from its elements d = 16 qg + 64 h + [0, 16) and returns the
-// factor of its scores (NaN for a column that is not finite). Cross-lane.
+// Elements 4 w + [0, 4) of chunk h of the columns (`own`), from the lane's elements of all
+// chunks (`raw`, for the column's maximum). Cross-lane.
 template <typename QT, int D>
-__device__ __forceinline__ float half_query(const QueryColumn<QT, D>& raw, bool valid, float scale,
-                                            HalfQuery<QT, D>& q) {
-  float x[D / 64][16];
+__device__ __forceinline__ void share_query(const QueryColumn<QT, D>& raw, const QT (&own)[4], int h,
+                                            int w, bool valid, float scale, int lane,
+                                            SharedQuery<QT, D>& q) {
   float mx = 0.f;
 #pragma unroll
-  for (int h = 0; h < D / 64; ++h) {
-    const QT* e = reinterpret_cast<const QT*>(raw.w[h]);
+  for (int c = 0; c < D / 64; ++c) {
+    const QT* e = reinterpret_cast<const QT*>(raw.w[c]);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      x[h][i] = valid ? to_float<QT>(e[i]) : 0.f;
-      mx = vmax(mx, fabsf(x[h][i]));  // NaN-propagating
-    }
+    for (int i = 0; i < 16; ++i) mx = vmax(mx, fabsf(to_float<QT>(e[i])));  // NaN-propagating
   }
   mx = vmax(mx, shfl_xor(mx, 16));
   mx = vmax(mx, shfl_xor(mx, 32));
+  mx = valid ? mx : 0.f;
   const bool finite = __builtin_isfinite(mx);
-  int ex = 15;
-  if (finite && mx > 0.f) frexpf(mx, &ex);
-  ex = max(ex - 15, -126);
+  float x[4];
 #pragma unroll
-  for (int h = 0; h < D / 64; ++h)
+  for (int i = 0; i < 4; ++i) x[i] = valid && finite ? to_float<QT>(own[i]) : 0.f;
+  float factor;
+  if constexpr (KF == kInt8) {
+    factor = scale * (mx / (float)kQRange);
+    // kQRange / mx overflows for mx below 2^-114: such columns are lifted by 2^64 (exact)
+    const float up = mx > 0.f && mx < 0x1p-64f ? 0x1p64f : 1.f;
+    const float inv = finite && mx > 0.f ? (float)kQRange / (mx * up) : 0.f;
+    uint32_t b[3][4];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float v = ldexpf(x[h][i], -ex);
-      const _Float16 hi = (_Float16)v;
-      q.op[0][2 * h + i / 8][i % 8] = hi;
-      if constexpr (HalfQuery<QT, D>::kTerms == 2)
-        q.op[1][2 * h + i / 8][i % 8] = (_Float16)(v - (float)hi);
+    for (int i = 0; i < 4; ++i) {
+      const QueryTerms t = query_terms(x[i] * up, inv);
+      b[0][i] = __builtin_bit_cast(uint32_t, t.hi);
+      b[1][i] = __builtin_bit_cast(uint32_t, t.lo);
+      b[2][i] = __builtin_bit_cast(uint32_t, t.lo2);
     }
-  return finite ? ldexpf(1.f, ex) * scale * code_scale<KF>() : __builtin_nanf("");
+#pragma unroll
+    for (int t = 0; t < 3; ++t)
+      reinterpret_cast<uint32_t*>(&q.op[q.at(t, h, 0)][lane])[w] = low_bytes(b[t]);
+  } else {
+    int ex = 15;
+    if (finite && mx > 0.f) frexpf(mx, &ex);
+    ex = max(ex - 15, -126);
+    factor = ldexpf(1.f, ex) * scale * code_scale<KF>();
+    half4_t op[2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float v = ldexpf(x[i], -ex);
+      op[0][i] = (_Float16)v;
+      op[1][i] = (_Float16)(v - (float)op[0][i]);
+    }
+#pragma unroll
+    for (int t = 0; t < SharedQuery<QT, D>::kTerms; ++t)
+      reinterpret_cast<uint2*>(&q.op[q.at(t, h, w / 2)][lane])[w % 2] =
+          __builtin_bit_cast(uint2, op[t]);
+  }
+  if (h == 0 && w == 0 && lane < 16) q.factor[lane] = finite ? factor : __builtin_nanf("");
 }
-
-template <typename QT, int D>
-__device__ __forceinline__ float make_query(const QueryColumn<QT, D>& raw, bool valid, float scale,
-                                            QkOperand<D, kInt8>& q) {
-  return query_column_i8<QT, D>(raw, valid, scale, q.hi, q.lo, q.lo2);
-}
-template <typename QT, int D>
-__device__ __forceinline__ float make_query(const QueryColumn<QT, D>& raw, bool valid, float scale,
-                                            HalfQuery<QT, D>& q) {
-  return half_query<QT, D>(raw, valid, scale, q);
-}
-template <typename QT, int D>
-using QueryOp = std::conditional_t<KF == kInt8, QkOperand<D, kInt8>, HalfQuery<QT, D>>;
 
 // The unit 2^e of the V scales: weights enter the output's products as p * (v_scale * 2^-e)
 // in f16, the accumulators hold the output times 2^-e. The first block's largest scale sets
@@ -104,12 +121,14 @@ struct VUnit {
 // head r; raw scores of keys outside [lo, hi) and of padding keys are -inf. `scores` (WEIGHTS):
 // where the lane's four scores go.
 template <typename QT, int D, bool WEIGHTS>
-__device__ __forceinline__ void bounded_block(const char* st, const QueryOp<QT, D>& q, float cf,
-                                              int tok_base, int lo, int hi, bool gvalid, int r,
+__device__ __forceinline__ void bounded_block(const char* st,
+                                              const int4_t (&q)[SharedQuery<QT, D>::kOps],
+                                              float cf, int tok_base, int lo, int hi, bool gvalid, int r,
                                               int qg, float4_t (&acc)[D / 16], float& m, float& l,
                                               VUnit& vu, bool& bad_score, bool masks,
                                               float* scores) {
   using S = Stage<D>;
+  using Q = SharedQuery<QT, D>;
   constexpr int KCH = D / 64, VB = D / 16, NPV = D / 16;
   const float4_t vs = *reinterpret_cast<const float4_t*>(st + S::kS + 64 + 16 * qg) * code_scale<KF>();
   const float4_t ks = *reinterpret_cast<const float4_t*>(st + S::kS + 16 * qg);
@@ -122,12 +141,12 @@ __device__ __forceinline__ void bounded_block(const char* st, const QueryOp<QT, 
     for (int h = 0; h < KCH; ++h)
       kop[h] = *reinterpret_cast<const int4_t*>(st + S::kK + k_chunk<D>(r, qg + 4 * h));
 #pragma unroll
-    for (int h = 0; h < KCH; ++h) si = __builtin_amdgcn_mfma_i32_16x16x64_i8(kop[h], q.hi[h], si, 0, 0, 0);
+    for (int h = 0; h < KCH; ++h) si = __builtin_amdgcn_mfma_i32_16x16x64_i8(kop[h], q[Q::at(0, h, 0)], si, 0, 0, 0);
 #pragma unroll
-    for (int h = 0; h < KCH; ++h) sf = __builtin_amdgcn_mfma_i32_16x16x64_i8(kop[h], q.lo2[h], sf, 0, 0, 0);
+    for (int h = 0; h < KCH; ++h) sf = __builtin_amdgcn_mfma_i32_16x16x64_i8(kop[h], q[Q::at(2, h, 0)], sf, 0, 0, 0);
     si = si << 7;
 #pragma unroll
-    for (int h = 0; h < KCH; ++h) si = __builtin_amdgcn_mfma_i32_16x16x64_i8(kop[h], q.lo[h], si, 0, 0, 0);
+    for (int h = 0; h < KCH; ++h) si = __builtin_amdgcn_mfma_i32_16x16x64_i8(kop[h], q[Q::at(1, h, 0)], si, 0, 0, 0);
 #pragma unroll
     for (int j = 0; j < 4; ++j) s4[j] = __builtin_fmaf((float)sf[j], 1.f / 128.f, (float)si[j]);
   } else {
@@ -142,8 +161,9 @@ __device__ __forceinline__ void bounded_block(const char* st, const QueryOp<QT, 
         codes_to_f16<KF>(sub ? c.w : c.y, p2, p3);
         const half8_t kop = {p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
 #pragma unroll
-        for (int t = 0; t < HalfQuery<QT, D>::kTerms; ++t)
-          s4 = __builtin_amdgcn_mfma_f32_16x16x32_f16(kop, q.op[t][2 * h + sub], s4, 0, 0, 0);
+        for (int t = 0; t < Q::kTerms; ++t)
+          s4 = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+              kop, __builtin_bit_cast(half8_t, q[Q::at(t, h, sub)]), s4, 0, 0, 0);
       }
     }
   }
@@ -280,7 +300,12 @@ __device__ __forceinline__ float log_sum(float m, float l) {
 template <int D, int NW>
 struct BoundedLds {
   static constexpr int kStageBytes = NW * Stage<D>::kBytes;
-  static constexpr int kMergeBytes = NW * 16 * (D + 2) * 4;
+  // a wave's outputs of a head: four lanes' runs of D / 4, each padded by four floats against
+  // bank conflicts (with single stores at stride D / 4, 1.8 us of a 12.3 us call); groups of 16
+  // heads, which would then take more LDS than the stages, go without the padding
+  __device__ static constexpr int run(int group) { return group == 16 ? D / 4 : D / 4 + 4; }
+  static constexpr int kMergeBytes =
+      NW * (16 * (D + 2) > 8 * (D + 16) + 32 ? 16 * (D + 2) : 8 * (D + 16) + 32) * 4;
   static constexpr int kBytes = 2 * kStageBytes > kMergeBytes ? 2 * kStageBytes : kMergeBytes;
 };
 
@@ -290,7 +315,9 @@ __global__ __launch_bounds__(NW * kWave) void bounded_decode_kernel(BoundedArgs 
   using S = Stage<D>;
   using L = BoundedLds<D, NW>;
   constexpr int NPV = D / 16, VB = D / 16;
+  static_assert(L::kBytes + sizeof(SharedQuery<QT, D>) + 64 <= 160 * 1024, "LDS");
   __shared__ __attribute__((aligned(16))) char lds[L::kBytes];
+  __shared__ SharedQuery<QT, D> query;
   __shared__ float lse[16];
 
   const int part = blockIdx.x, kvh = blockIdx.y, seq = blockIdx.z;
@@ -302,7 +329,17 @@ __global__ __launch_bounds__(NW * kWave) void bounded_decode_kernel(BoundedArgs 
   const int tok = decode_token(a, seq);
   if (tok < 0) return;  // not a decode row
   QueryColumn<QT, D> raw;
-  load_query_column<QT, D>(query_col_ptr<QT>(a, tok, kvh * G + (gvalid ? r : 0), qg), raw);
+  const QT* const qp = query_col_ptr<QT>(a, tok, kvh * G + (gvalid ? r : 0), qg);
+  load_query_column<QT, D>(qp, raw);
+  constexpr int kQuads = D / 16;  // of a lane; wave w builds those w, w + NW, ...
+  struct alignas(4 * sizeof(QT)) Quad {
+    QT e[4];
+  } own[(kQuads + NW - 1) / NW];
+#pragma unroll
+  for (int i = 0; i < (kQuads + NW - 1) / NW; ++i) {
+    const int quad = min(wave + i * NW, kQuads - 1);
+    own[i] = *reinterpret_cast<const Quad*>(qp + 64 * (quad / 4) + 4 * (quad % 4));
+  }
   const bool reporter = part == 0 && kvh == 0 && threadIdx.x == 0;
   const VisibleList v = visible_list(a, bounded_ctx(a, a.context_lens[seq], reporter));
   const int parts = row_parts(a, v);
@@ -321,8 +358,18 @@ __global__ __launch_bounds__(NW * kWave) void bounded_decode_kernel(BoundedArgs 
   if (0 < nblk) stage_block<D>(a, __builtin_amdgcn_readlane(ids, 0), kvh, lane, st0);
   if (1 < nblk) stage_block<D>(a, __builtin_amdgcn_readlane(ids, 1), kvh, lane, st1);
 
-  QueryOp<QT, D> q;
-  const float cf = make_query<QT, D>(raw, gvalid, a.qk_scale_log2, q);
+  // (the blocks' loads are on their way)
+#pragma unroll
+  for (int i = 0; i < (kQuads + NW - 1) / NW; ++i) {
+    const int quad = wave + i * NW;
+    if (quad < kQuads)
+      share_query<QT, D>(raw, own[i].e, quad / 4, quad % 4, gvalid, a.qk_scale_log2, lane, query);
+  }
+  __syncthreads();
+  int4_t q[SharedQuery<QT, D>::kOps];
+#pragma unroll
+  for (int i = 0; i < SharedQuery<QT, D>::kOps; ++i) q[i] = query.op[i][lane];
+  const float cf = query.factor[r];
   float4_t acc[NPV];
 #pragma unroll
   for (int n = 0; n < NPV; ++n) acc[n] = float4_t{0.f, 0.f, 0.f, 0.f};
@@ -365,28 +412,33 @@ __global__ __launch_bounds__(NW * kWave) void bounded_decode_kernel(BoundedArgs 
   __syncthreads();
   float* const sm = reinterpret_cast<float*>(lds);  // [NW][16]
   float* const sl = sm + NW * 16;
-  float* const so = sl + NW * 16;  // [NW][G][D]
+  const int run = L::run(G);
+  float* const so = sl + NW * 16;  // [NW][G][4][run]
   if (gvalid) {
     if (qg == 0) {
       sm[wave * 16 + r] = m;
       sl[wave * 16 + r] = l;
     }
-    float* o = so + (wave * G + r) * D + VB * 4 * qg;
+    float* o = so + ((wave * G + r) * 4 + qg) * run;  // d = D / 4 qg + t
 #pragma unroll
-    for (int n = 0; n < NPV; ++n)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) o[VB * j + n] = acc[n][j] * up;
+    for (int t = 0; t < D / 4; t += 4)
+      *reinterpret_cast<float4_t*>(o + t) =
+          float4_t{acc[t % VB][t / VB], acc[(t + 1) % VB][(t + 1) / VB],
+                   acc[(t + 2) % VB][(t + 2) / VB], acc[(t + 3) % VB][(t + 3) / VB]} * up;
   }
   __syncthreads();
   for (int i = threadIdx.x; i < G * D; i += NW * kWave) {
     const int g = i / D, d = i % D;
+    const float* o = so + (g * 4 + d / (D / 4)) * run + d % (D / 4);
     float M = -FLT_MAX;
+#pragma unroll
     for (int w = 0; w < NW; ++w) M = fmaxf(M, sm[w * 16 + g]);
     float Lg = 0.f, O = 0.f;
+#pragma unroll
     for (int w = 0; w < NW; ++w) {
       const float f = __builtin_amdgcn_exp2f(sm[w * 16 + g] - M);
       Lg = fmaf(sl[w * 16 + g], f, Lg);
-      O = fmaf(so[(w * G + g) * D + d], f, O);
+      O = fmaf(o[w * G * 4 * run], f, O);
     }
     const int h = kvh * G + g;
     if (parts == 1) {
@@ -485,9 +537,11 @@ int launch(const BoundedArgs& a, hipStream_t stream) {
 template <typename QT, int D>
 int launch_dim(const BoundedArgs& a, hipStream_t s) {
   const bool weights = a.kw.values != nullptr;
-  constexpr int W = wide_waves(D);
-  // total_waves: the workgroup's waves, four or wide_waves()
-  if (a.total_waves == W) return weights ? launch<QT, D, W, true>(a, s) : launch<QT, D, W, false>(a, s);
+  // total_waves: the workgroup's waves
+  if constexpr (wide_waves(D) == 16) {
+    if (a.total_waves == 16) return weights ? launch<QT, D, 16, true>(a, s) : launch<QT, D, 16, false>(a, s);
+  }
+  if (a.total_waves == 8) return weights ? launch<QT, D, 8, true>(a, s) : launch<QT, D, 8, false>(a, s);
   return weights ? launch<QT, D, 4, true>(a, s) : launch<QT, D, 4, false>(a, s);
 }
 

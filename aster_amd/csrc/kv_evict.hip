@@ -10,6 +10,8 @@
 // lane. In place a token's destination lies at or before its source, and tokens before the
 // source's: a workgroup goes through them in order, a batch of rows loaded before any of it is
 // stored. Into other pages the batches are independent workgroups.
+#include <climits>
+
 #include "attention_common.h"
 
 namespace astr {
@@ -70,38 +72,252 @@ __device__ __forceinline__ int64_t row_of(const EvictArgs& a, const int32_t* row
   return row;
 }
 
+// What a select workgroup works on.
+struct Segment {
+  int n;                   // tokens
+  int64_t src_row, dst_row;  // -1: nothing moves
+  const float* w;
+  float* w_dst;
+  const int32_t* table;
+  int32_t* kept;
+  bool reporter;           // of the row's faults and length
+  __device__ __forceinline__ explicit Segment(const EvictArgs& a) {
+    const int head = blockIdx.x, layer = blockIdx.y, seq = blockIdx.z;
+    reporter = head == 0 && layer == 0 && threadIdx.x == 0;
+    n = evict_ctx(a, seq, reporter);
+    src_row = row_of(a, a.rows, seq, reporter);
+    dst_row = row_of(a, a.dst_rows, seq, reporter);
+    w = a.weights + src_row * a.w_row + layer * a.w_layer + head * a.w_head;
+    w_dst = a.weights + dst_row * a.w_row + layer * a.w_layer + head * a.w_head;
+    table = a.tables + (int64_t)seq * a.t_stride;
+    kept = a.kept + (((int64_t)seq * gridDim.y + layer) * gridDim.x + head) * a.keep;
+  }
+  __device__ __forceinline__ bool real(const EvictArgs& a, int t) const {
+    const int id = table[t / kBlockTokens];
+    return (unsigned)id < (unsigned)a.cache.num_blocks &&
+           a.cache.key_valid[(int64_t)id * kBlockTokens + t % kBlockTokens] != 0;
+  }
+  // Ends a segment of which `keep` tokens stay.
+  template <int T>
+  __device__ __forceinline__ void finish(const EvictArgs& a, int keep) const {
+    for (int i = keep + (int)threadIdx.x; i < a.keep; i += T) kept[i] = -1;
+    if (reporter) a.new_lens[blockIdx.z] = keep;
+  }
+};
+
+// One pass of the radix select by T threads: hist holds the counts of the digit's values; finds
+// the value of the `need`-th largest and how many of that value are among the `need`: found[0],
+// found[1]. Every thread calls it, after a barrier.
+template <int T>
+__device__ __forceinline__ void find_digit(const int* hist, int need, int* wave_sum, int* found) {
+  constexpr int kPer = kBins / T;  // consecutive bins a thread holds, from the top down
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int bin0 = kPer * (T - 1 - (int)threadIdx.x);
+  int c[kPer], incl = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    c[i] = hist[bin0 + i];
+    incl += c[i];
+  }
+  int above = -incl;
+#pragma unroll
+  for (int off = 1; off < kWave; off <<= 1) {
+    const int v = __shfl_up(incl, off, kWave);
+    if (lane >= off) incl += v;
+  }
+  if (lane == kWave - 1) wave_sum[wave] = incl;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < T / kWave; ++i) incl += i < wave ? wave_sum[i] : 0;
+  above += incl;
+  if (above < need && incl >= need) {  // one thread
+    int bin = bin0 + kPer - 1;
+#pragma unroll
+    for (int i = kPer - 1; i > 0; --i)
+      if (bin == bin0 + i && above + c[i] < need) {
+        above += c[i];
+        --bin;
+      }
+    found[0] = bin;
+    found[1] = need - above;
+  }
+  __syncthreads();
+}
+
+// Segments of up to R * T tokens: thread i holds the bits of tokens i, i + T, ... in registers,
+// read once; order comes from one prefix over the counts of all (round, wave) pairs.
+// Bound by the chain of barriers and LDS round trips of a segment, so that a CU holds as many
+// segments as it can: 256 threads up to 12288 tokens. 8 prompts of 1500 to 9000 tokens, 16 layers,
+// 8 heads: TIME_SELECT us; 58 with 1024 threads, 72 when every pass read the weights again and
+// every round of the last one waited for the one before.
+template <int T, int R>
+__global__ __launch_bounds__(T) void select_held_kernel(EvictArgs a) {
+  constexpr int kWavesT = T / kWave, kPairs = R * kWavesT;
+  __shared__ __attribute__((aligned(16))) int hist[kBins];
+  __shared__ int count_a[kPairs], count_b[kPairs];
+  __shared__ int wave_sum[kWavesT], found[2], total;
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const Segment g(a);
+  if (g.src_row < 0 || g.dst_row < 0) return g.finish<T>(a, 0);
+  const int n = g.n, pairs = (n + T - 1) / T * kWavesT;
+
+  // The exclusive prefix of counts[round * kWavesT + wave] in place, by one wave; the sum in
+  // `total` where asked.
+  auto scan = [&](int* counts, int by, bool sum) __attribute__((always_inline)) {
+    if (wave != by) return;
+    int base = 0;
+    for (int c0 = 0; c0 < pairs; c0 += kWave) {
+      const int v = c0 + lane < pairs ? counts[c0 + lane] : 0;
+      int incl = v;
+#pragma unroll
+      for (int off = 1; off < kWave; off <<= 1) {
+        const int u = __shfl_up(incl, off, kWave);
+        if (lane >= off) incl += u;
+      }
+      if (c0 + lane < pairs) counts[c0 + lane] = base + incl - v;
+      base += __shfl(incl, kWave - 1, kWave);
+    }
+    if (sum && lane == 0) total = base;
+  };
+
+  uint32_t u[R];  // 0: no token, or a padding one
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int t = i * T + (int)threadIdx.x;
+    u[i] = t < n ? ordered(g.w[t]) : 0u;
+  }
+  uint64_t fixed = 0;  // bit i: token i stays for its place
+  int count = n;
+  if (a.cache.key_valid != nullptr) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      if (i * T < n) {  // (uniform)
+        const int t = i * T + (int)threadIdx.x;
+        if (u[i] != 0 && !g.real(a, t)) u[i] = 0;
+        const uint64_t b = __ballot(u[i] != 0);
+        if (lane == 0) count_a[i * kWavesT + wave] = __builtin_popcountll(b);
+      }
+    }
+    __syncthreads();
+    scan(count_a, 0, true);
+    __syncthreads();
+    count = total;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      if (i * T < n) {
+        const uint64_t b = __ballot(u[i] != 0);
+        const int rank = count_a[i * kWavesT + wave] + lanes_below(b, lane);
+        if (u[i] != 0 && (rank < a.sinks || rank >= count - a.recent)) fixed |= 1ull << i;
+      }
+    }
+    __syncthreads();  // count_a is written again
+  } else {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int t = i * T + (int)threadIdx.x;
+      if (t < n && (t < a.sinks || t >= n - a.recent)) fixed |= 1ull << i;
+    }
+  }
+  const int keep = min(a.keep, count);
+
+  // ---- the bits of the lightest of the heaviest, of which `ties` stay
+  uint32_t threshold = 0;
+  int ties = 0;
+  if (keep < count) {
+    // those of the others that stay (sinks + recent <= keep < count: the two do not overlap)
+    int need = keep - a.sinks - a.recent;
+    threshold = 0xffffffffu;
+    if (need > 0) {
+      uint32_t prefix = 0, known = 0;
+#pragma unroll 1
+      for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
+#pragma unroll
+        for (int i = 0; i < kBins / T / 4 + (kBins / T < 4); ++i)
+          if ((i * T + (int)threadIdx.x) * 4 < kBins)
+            *reinterpret_cast<int4_t*>(hist + (i * T + (int)threadIdx.x) * 4) = int4_t{0, 0, 0, 0};
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+          if (u[i] != 0 && !(fixed >> i & 1) && (u[i] & known) == prefix)
+            atomicAdd(&hist[u[i] >> shift & (bins - 1)], 1);
+        __syncthreads();
+        find_digit<T>(hist, need, wave_sum, found);
+        prefix |= (uint32_t)found[0] << shift;
+        known |= (uint32_t)(bins - 1) << shift;
+        need = found[1];
+      }
+      threshold = prefix;
+      ties = need;
+    }
+  }
+
+  // ---- the tokens that stay, in order
+  const bool all = keep == count;
+  auto more_of = [&](int i) __attribute__((always_inline)) -> bool {
+    return u[i] != 0 && (all || (fixed >> i & 1) || u[i] > threshold);
+  };
+  auto tie_of = [&](int i) __attribute__((always_inline)) -> bool {
+    return u[i] == threshold && !more_of(i) && u[i] != 0;
+  };
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    if (i * T < n) {
+      const uint64_t bm = __ballot(more_of(i)), bt = __ballot(tie_of(i));
+      if (lane == 0) {
+        count_a[i * kWavesT + wave] = __builtin_popcountll(bm);
+        count_b[i * kWavesT + wave] = __builtin_popcountll(bt);
+      }
+    }
+  }
+  __syncthreads();
+  scan(count_a, 0, false);
+  scan(count_b, 1, false);
+  __syncthreads();
+  // in place, a weight's destination may be another thread's source: all are read before any is
+  // stored (u becomes the weight's own bits)
+  int at[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    at[i] = INT_MAX;
+    if (i * T < n) {
+      const bool more = more_of(i), tie = tie_of(i);
+      const uint64_t bm = __ballot(more), bt = __ballot(tie);
+      const int m = count_a[i * kWavesT + wave] + lanes_below(bm, lane);
+      const int e = count_b[i * kWavesT + wave] + lanes_below(bt, lane);
+      if (more || (tie && e < ties)) at[i] = m + min(e, ties);
+      if (at[i] < keep) u[i] = __builtin_bit_cast(uint32_t, g.w[i * T + (int)threadIdx.x]);
+    }
+  }
+  wait_vmcnt<0>();
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    if (at[i] < keep) {  // (and so below a.keep)
+      g.kept[at[i]] = i * T + (int)threadIdx.x;
+      g.w_dst[at[i]] = __builtin_bit_cast(float, u[i]);
+    }
+  }
+  g.finish<T>(a, keep);
+}
+
+// Segments of any length: every pass reads the weights again.
 __global__ __launch_bounds__(kThreads) void select_kernel(EvictArgs a) {
   __shared__ int hist[kBins];
   __shared__ int wave_a[kBlockWaves], wave_b[kBlockWaves];
-  __shared__ int found[3];
-  const int head = blockIdx.x, layer = blockIdx.y, seq = blockIdx.z;
+  __shared__ int found[2];
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const int layers = gridDim.y, heads = gridDim.x;
-  const bool reporter = head == 0 && layer == 0 && threadIdx.x == 0;
-  const int n = evict_ctx(a, seq, reporter);
-  const int64_t src_row = row_of(a, a.rows, seq, reporter);
-  const int64_t dst_row = row_of(a, a.dst_rows, seq, reporter);
-  int32_t* const kept = a.kept + (((int64_t)seq * layers + layer) * heads + head) * a.keep;
-  if (src_row < 0 || dst_row < 0) {  // nothing moves
-    for (int i = threadIdx.x; i < a.keep; i += kThreads) kept[i] = -1;
-    if (reporter) a.new_lens[seq] = 0;
-    return;
-  }
-  const float* const w = a.weights + src_row * a.w_row + layer * a.w_layer + head * a.w_head;
-  float* const w_dst = a.weights + dst_row * a.w_row + layer * a.w_layer + head * a.w_head;
-  const int32_t* const table = a.tables + (int64_t)seq * a.t_stride;
-  const uint8_t* const valid = a.cache.key_valid;
-  auto real = [&](int t) __attribute__((always_inline)) -> bool {
-    if (valid == nullptr) return true;
-    const int id = table[t / kBlockTokens];
-    return (unsigned)id < (unsigned)a.cache.num_blocks &&
-           valid[(int64_t)id * kBlockTokens + t % kBlockTokens] != 0;
-  };
+  const Segment g(a);
+  if (g.src_row < 0 || g.dst_row < 0) return g.finish<kThreads>(a, 0);
+  const int n = g.n;
+  const float* const w = g.w;
+  const bool masks = a.cache.key_valid != nullptr;
+  auto real = [&](int t) __attribute__((always_inline)) -> bool { return !masks || g.real(a, t); };
 
   // ---- how many real tokens there are, and which ones stay for their place: those before
   // `sink_end` and from `recent_begin` on
   int count = n, sink_end = min(a.sinks, n), recent_begin = max(0, n - a.recent);
-  if (valid != nullptr) {
+  if (masks) {
     count = 0;
     for (int t0 = 0; t0 < n; t0 += kThreads) {
       const int t = t0 + (int)threadIdx.x;
@@ -160,24 +376,7 @@ __global__ __launch_bounds__(kThreads) void select_kernel(EvictArgs a) {
           if ((u & known) == prefix) atomicAdd(&hist[u >> shift & (bins - 1)], 1);
         }
         __syncthreads();
-        // counts from the top: thread i holds bins 2 i' and 2 i' + 1, i' = kThreads - 1 - i
-        const int i2 = 2 * (kThreads - 1 - (int)threadIdx.x);
-        const int hi = hist[i2 + 1], lo = hist[i2];
-        int incl = hi + lo;
-        for (int off = 1; off < kWave; off <<= 1) {
-          const int v = __shfl_up(incl, off, kWave);
-          if (lane >= off) incl += v;
-        }
-        if (lane == kWave - 1) wave_a[wave] = incl;
-        __syncthreads();
-        for (int i = 0; i < wave; ++i) incl += wave_a[i];
-        const int above = incl - hi - lo;
-        if (above < need && incl >= need) {  // one thread
-          const bool in_hi = above + hi >= need;
-          found[0] = in_hi ? i2 + 1 : i2;
-          found[1] = need - (in_hi ? above : above + hi);
-        }
-        __syncthreads();
+        find_digit<kThreads>(hist, need, wave_a, found);
         prefix |= (uint32_t)found[0] << shift;
         known |= (uint32_t)(bins - 1) << shift;
         need = found[1];
@@ -218,20 +417,26 @@ __global__ __launch_bounds__(kThreads) void select_kernel(EvictArgs a) {
     if (more || (tie && e < ties)) {
       const int at = m + min(e, ties);
       if (at < keep) {  // (always, unless key_valid or the weights change under the kernel)
-        kept[at] = t;
-        w_dst[at] = weight;  // at <= t: in place, read by now
+        g.kept[at] = t;
+        g.w_dst[at] = weight;  // at <= t: in place, read by now
       }
     }
     __syncthreads();
   }
-  for (int i = keep + (int)threadIdx.x; i < a.keep; i += kThreads) kept[i] = -1;
-  if (reporter) a.new_lens[seq] = keep;
+  g.finish<kThreads>(a, keep);
 }
+
+// Rows of a batch: kMoveDepth a thread, whose three loads in a row (the token, its pages, its
+// bytes) are on their way together.
+constexpr int kMoveDepth = 4;
+template <int D>
+constexpr int move_rows() { return kMoveDepth * kThreads / (D / 16); }
 
 // IN_PLACE: one workgroup goes through all batches of its rows, else blockIdx.x names one.
 template <int D, bool IN_PLACE>
 __global__ __launch_bounds__(kThreads) void move_kernel(EvictArgs a) {
-  constexpr int kLanes = D / 16, kRows = kThreads / kLanes;  // lanes a row, rows a batch
+  constexpr int kLanes = D / 16;           // a row's
+  constexpr int kRows = move_rows<D>(), kStep = kThreads / kLanes;
   const int heads = a.cache.num_kv_heads, layers = gridDim.y;
   const int batches = (a.keep + kRows - 1) / kRows;
   const int first = IN_PLACE ? 0 : blockIdx.x % batches;
@@ -249,47 +454,65 @@ __global__ __launch_bounds__(kThreads) void move_kernel(EvictArgs a) {
   const int new_len = a.new_lens[seq];
   bool bad = false;
   for (int batch = first; batch < (IN_PLACE ? batches : first + 1); ++batch) {
-    const int j = batch * kRows + row;
     if (batch * kRows >= new_len) break;
-    const int t = j < new_len ? kept[j] : -1;
-    int src = -1, dst = -1;
-    if (t >= 0) {
-      src = src_table[t / kBlockTokens];
-      dst = dst_table[j / kBlockTokens];
-      if ((unsigned)src >= (unsigned)a.cache.num_blocks ||
-          (unsigned)dst >= (unsigned)a.cache.num_blocks) {
-        bad = true;
-        src = -1;
-      } else if (IN_PLACE && t == j) {
-        src = -1;  // stays where it is
+    int t[kMoveDepth], src[kMoveDepth], dst[kMoveDepth];
+    typedef uint32_t word4_t __attribute__((ext_vector_type(4)));
+    word4_t v[kMoveDepth];
+    float s[kMoveDepth];
+#pragma unroll
+    for (int i = 0; i < kMoveDepth; ++i) {
+      const int j = batch * kRows + i * kStep + row;
+      t[i] = j < new_len ? kept[j] : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < kMoveDepth; ++i) {
+      const int j = batch * kRows + i * kStep + row;
+      src[i] = dst[i] = -1;
+      v[i] = word4_t{0, 0, 0, 0};
+      s[i] = 0.f;
+      if (t[i] >= 0) {
+        src[i] = src_table[t[i] / kBlockTokens];
+        dst[i] = dst_table[j / kBlockTokens];
       }
     }
-    uint4 v;
-    float s = 0.f;
-    if (src >= 0) {
-      v = *reinterpret_cast<const uint4*>(codes + src * a.cache.code_block_stride +
-                                          t % kBlockTokens * D + part * 16);
-      if (part == 0) s = scales[src * a.cache.scale_block_stride + t % kBlockTokens];
+#pragma unroll
+    for (int i = 0; i < kMoveDepth; ++i) {
+      const int j = batch * kRows + i * kStep + row;
+      if (t[i] >= 0 && ((unsigned)src[i] >= (unsigned)a.cache.num_blocks ||
+                        (unsigned)dst[i] >= (unsigned)a.cache.num_blocks)) {
+        bad = true;
+        src[i] = -1;
+      }
+      if (IN_PLACE && t[i] == j) src[i] = -1;  // stays where it is
+      if (src[i] >= 0) {
+        v[i] = *reinterpret_cast<const word4_t*>(codes + src[i] * a.cache.code_block_stride +
+                                               t[i] % kBlockTokens * D + part * 16);
+        if (part == 0) s[i] = scales[src[i] * a.cache.scale_block_stride + t[i] % kBlockTokens];
+      }
     }
     if constexpr (IN_PLACE) {
       wait_vmcnt<0>();  // every load of the batch has returned before a store of it goes out
       __syncthreads();
     }
-    if (src >= 0) {
-      *reinterpret_cast<uint4*>(codes + dst * a.cache.code_block_stride + j % kBlockTokens * D +
-                                part * 16) = v;
-      if (part == 0) scales[dst * a.cache.scale_block_stride + j % kBlockTokens] = s;
+#pragma unroll
+    for (int i = 0; i < kMoveDepth; ++i) {
+      const int j = batch * kRows + i * kStep + row;
+      if (src[i] >= 0) {
+        *reinterpret_cast<word4_t*>(codes + dst[i] * a.cache.code_block_stride +
+                                  j % kBlockTokens * D + part * 16) = v[i];
+        if (part == 0) scales[dst[i] * a.cache.scale_block_stride + j % kBlockTokens] = s[i];
+      }
+      if (a.cache.key_valid != nullptr && which == 0 && layer == 0 && part == 0 && t[i] >= 0 &&
+          (unsigned)dst[i] < (unsigned)a.cache.num_blocks)
+        a.cache.key_valid[(int64_t)dst[i] * kBlockTokens + j % kBlockTokens] = 1;
     }
-    if (a.cache.key_valid != nullptr && which == 0 && layer == 0 && part == 0 && t >= 0 &&
-        (unsigned)dst < (unsigned)a.cache.num_blocks)
-      a.cache.key_valid[(int64_t)dst * kBlockTokens + j % kBlockTokens] = 1;
   }
   if (bad) atomicOr(a.err_flag, ASTR_FLAG_BAD_INDEX);
 }
 
 template <int D>
 void launch_move(const EvictArgs& a, int layers, hipStream_t stream) {
-  constexpr int kRows = kThreads / (D / 16);
+  constexpr int kRows = move_rows<D>();
   const uint32_t units = 2u * (uint32_t)a.cache.num_kv_heads;
   if (a.dst_tables == nullptr) {
     hipLaunchKernelGGL((move_kernel<D, true>), dim3(units, layers, a.num_seqs), dim3(kThreads), 0,
@@ -383,8 +606,17 @@ extern "C" int astr_kv_evict(const astr_paged_kv* cache, int32_t num_layers,
   const int64_t batches = ((int64_t)keep * (D / 16) + kThreads - 1) / kThreads;
   if (2 * batches * cache->num_kv_heads > INT32_MAX)
     return fail(ASTR_EUNSUPPORTED, "keep %d too large for one launch", keep);
-  hipLaunchKernelGGL(select_kernel, dim3(cache->num_kv_heads, num_layers, num_seqs), dim3(kThreads),
-                     0, s, a);
+  const dim3 segments(cache->num_kv_heads, num_layers, num_seqs);
+  if (max_context_len <= 8 * 256)
+    hipLaunchKernelGGL((select_held_kernel<256, 8>), segments, dim3(256), 0, s, a);
+  else if (max_context_len <= 16 * 256)
+    hipLaunchKernelGGL((select_held_kernel<256, 16>), segments, dim3(256), 0, s, a);
+  else if (max_context_len <= 48 * 256)
+    hipLaunchKernelGGL((select_held_kernel<256, 48>), segments, dim3(256), 0, s, a);
+  else if (max_context_len <= 32 * kThreads)
+    hipLaunchKernelGGL((select_held_kernel<kThreads, 32>), segments, dim3(kThreads), 0, s, a);
+  else
+    hipLaunchKernelGGL(select_kernel, segments, dim3(kThreads), 0, s, a);
   if (D == 64) launch_move<64>(a, num_layers, s);
   else if (D == 128) launch_move<128>(a, num_layers, s);
   else launch_move<256>(a, num_layers, s);

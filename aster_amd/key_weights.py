@@ -38,9 +38,17 @@ class KeyWeightRows:
             raise ValueError("Key weight rows of one batch must be distinct")
         self.weights, self.rows = weights, tuple(rows)
         self.table = torch.tensor(rows, dtype=torch.int32).to(weights.values.device)
+        v = weights.values
+        self._descs = [_native.KeyWeightsDesc(
+            values=v[0, layer].data_ptr(), row_stride=v.stride(0), head_stride=v.stride(2),
+            rows=self.table.data_ptr(), num_rows=weights.rows, capacity=weights.capacity)
+            for layer in range(v.shape[1])]
 
     def __len__(self):
         return len(self.rows)
+
+    def desc(self, layer):
+        return self._descs[layer]
 
 
 class KeyWeights:
@@ -69,12 +77,6 @@ class KeyWeights:
             raise ValueError(f"{what} were made for another cache layout")
         if len(selected) != num_seqs:
             raise ValueError(f"{what} must have one row per sequence")
-
-    def desc(self, selected, layer=0):
-        v = self.values
-        return _native.KeyWeightsDesc(
-            values=v[0, layer].data_ptr(), row_stride=v.stride(0), head_stride=v.stride(2),
-            rows=selected.table.data_ptr(), num_rows=self.rows, capacity=self.capacity)
 
 
 def require_rows(cache, selected, num_seqs, what="key_weights"):

@@ -27,6 +27,7 @@ with one launch over all rows.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 
@@ -67,6 +68,7 @@ class PagedKVCache:
         self.has_padding = False  # some slot may hold a padding key (descriptors carry key_valid)
         self.err_flag = torch.zeros(1, dtype=torch.int32, device=device)
         self._workspace = None
+        self._bounded_sizes = {}  # workspace bytes by a call's sizes (a call to the library each)
         self._descs = [self._make_desc(layer) for layer in range(num_layers)]
 
     # ---- descriptors --------------------------------------------------------
@@ -520,10 +522,24 @@ class PagedKVCache:
                                 sinks=None, key_weights=False, num_query_tokens=0, max_query_len=0):
         """Workspace of a call with ``sinks``, or of :meth:`paged_attention_weights`
         (``key_weights=True``); the last two arguments as the call's packed queries."""
-        return int(_native.lib().astr_paged_attention_i8_bounded_workspace_bytes(
-            num_seqs, num_q_heads, self.num_kv_heads, self.head_dim, _DTYPE_CODES[dtype],
-            num_query_tokens, max_query_len, max_context_len, window or 0, sinks or 0,
-            1 if key_weights else 0))
+        sizes = (num_seqs, num_q_heads, self.num_kv_heads, self.head_dim, _DTYPE_CODES[dtype],
+                 num_query_tokens, max_query_len, max_context_len, window or 0, sinks or 0,
+                 1 if key_weights else 0)
+        need = self._bounded_sizes.get(sizes)
+        if need is None:
+            with self._on_device():
+                need = int(_native.lib().astr_paged_attention_i8_bounded_workspace_bytes(*sizes))
+            if len(self._bounded_sizes) >= 1024:  # lengths change from step to step
+                self._bounded_sizes.clear()
+            self._bounded_sizes[sizes] = need
+        return need
+
+    def _on_device(self):
+        """Makes the arena's device current for a call to the library, which plans for and
+        launches on the current one."""
+        if self.device.index is None or self.device.index == torch.cuda.current_device():
+            return contextlib.nullcontext()
+        return torch.cuda.device(self.device)
 
     def _bounded_attention(self, layer, query, block_tables, context_lens, *, max_context_len,
                            scale=None, window=None, sinks=None, query_start_loc=None,
@@ -590,12 +606,11 @@ class PagedKVCache:
                 max_query_len, block_tables.data_ptr(), _row_stride(block_tables),
                 context_lens.data_ptr(), num_seqs, num_q_heads, max_context_len, scale]
         tail = [workspace.data_ptr() if need else None, need, self.err_flag.data_ptr(), stream]
-        with torch.cuda.device(self.device):
+        with self._on_device():
             if key_weights is None:
                 rc = lib.astr_paged_attention_i8_sinks(*args, window, sinks, *tail)
             else:
-                desc = key_weights.weights.desc(key_weights, layer)
-                rc = lib.astr_paged_attention_i8_key_weights(*args, ctypes.byref(desc), *tail)
+                rc = lib.astr_paged_attention_i8_key_weights(*args, key_weights.desc(layer), *tail)
         _native.check(rc, "paged_attention")
         if work is not None:
             prefill = packed and max_query_len > 1
@@ -648,12 +663,11 @@ class PagedKVCache:
         kept = torch.empty((num_seqs, self.num_layers, self.num_kv_heads, keep), dtype=torch.int32,
                            device=self.device)
         lengths = torch.empty((num_seqs,), dtype=torch.int32, device=self.device)
-        desc = weights.desc(key_weights)
         stream = torch.cuda.current_stream(self.device).cuda_stream
-        with torch.cuda.device(self.device):
+        with self._on_device():
             rc = _native.lib().astr_kv_evict(
                 self._descs[0], self.num_layers, self.codes.stride(1), self.scales.stride(1),
-                ctypes.byref(desc), weights.values.stride(1),
+                key_weights.desc(0), weights.values.stride(1),
                 into.table.data_ptr() if into is not None else None, block_tables.data_ptr(),
                 _row_stride(block_tables), dst_tables.data_ptr() if dst_tables is not None else None,
                 _row_stride(dst_tables) if dst_tables is not None else 0, context_lens.data_ptr(),
