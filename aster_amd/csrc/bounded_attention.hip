@@ -281,8 +281,9 @@ int bounded_attention(const Call& c) {
   chunk.pf_ws = static_cast<float*>(c.workspace);
   chunk.pf_bytes = need;
   chunk.sinks = c.sinks;
-  const int rc = w == nullptr && c.sinks > 0 ? launch_prefill_sinks(chunk, c.q_dtype, s)
-                                             : launch_prefill(chunk, c.q_dtype, s);
+  // (the build with sinks also rounds less for f16 and fp32 queries)
+  const int rc = c.sinks > 0 || c.q_dtype != ASTR_BF16 ? launch_prefill_sinks(chunk, c.q_dtype, s)
+                                                       : launch_prefill(chunk, c.q_dtype, s);
   if (rc != 0 || w == nullptr) return rc;
   a.chunk_ws = static_cast<float*>(c.workspace);
   a.min_rows = chunk.pf_min_rows;

@@ -50,6 +50,17 @@ constexpr int KF = ASTR_KF;  // this translation unit's code format
 constexpr bool kSinks = ASTR_PF_SINKS != 0;
 // The kernels' arguments. sinks_of is 0 without sinks, which leaves no code.
 using PrefillArgs = std::conditional_t<kSinks, SinkChunkArgs, ChunkArgs>;
+
+// How the V scales enter. Else (bf16 queries, and every query without sinks) V operands are
+// rounded products of code and scale and softmax weights are rounded to f16: three roundings of
+// 2^-11 per term, far below a bf16 output's own 2^-9 but above an f16 output's. Here, for f16 and
+// fp32 queries, the V operands are the codes, exactly, and the scale enters with the weight in
+// fp32, ahead of one rounding to f16 (two f16 terms for fp32 queries): errors of f16 outputs
+// against 64 bits 4.0e-4 -> 2.9e-4 (2.1e-4 is their own rounding). The product enters in units
+// of 2^ve: the largest V scale so far in [2^4, 2^7) of it, as weights are up to 2^8.
+template <typename QT>
+constexpr bool exact_v() { return kSinks && !std::is_same<QT, bf16_t>::value; }
+constexpr int kNoUnit = -120, kUnitBias = 128;
 __host__ __device__ __forceinline__ int sinks_of(const ChunkArgs& a) {
   if constexpr (kSinks) return static_cast<const SinkChunkArgs&>(a).sinks;
   else return 0;
@@ -386,6 +397,7 @@ struct PrefillLds {
   uint4 k[2][2 * kChunks * kWave];
   uint4 v[2][kWaves * kRowsN * kWave];
   __attribute__((aligned(16))) float ks[2][kWaves * kBlockTokens];
+  __attribute__((aligned(16))) float vs[kSinks ? 2 : 1][kSinks ? kWaves * kBlockTokens : 4];
   __attribute__((aligned(16))) uint32_t pad[2][kWaves * 4];
   __attribute__((aligned(16))) int flags[2][kWaves];
 };
@@ -446,7 +458,7 @@ __device__ __forceinline__ void load_raw(const AttnArgs& a, int id, int kvh, int
 // The wave's block into the operands of buffer `buf`, as block `w` of its step. The V
 // exponent e is the unit's current `ve`, or more where a scale exceeds `vlim` = 2^(15 + ve)
 // / format_max, so that every f16 product stays below 2^15.
-template <int D, bool kPad>
+template <int D, bool kPad, bool kExactV>
 __device__ __forceinline__ void convert_raw(const AttnArgs& a, const RawBlock<D>& b,
                                             PrefillLds<D>& L, int buf, int w, int lane, bool masks,
                                             int ve, float vlim) {
@@ -470,7 +482,21 @@ __device__ __forceinline__ void convert_raw(const AttnArgs& a, const RawBlock<D>
   constexpr float cs = v_weight_scale<KF>();
   int e = ve;
   float c = cs;
-  if (__ballot(vsm > vlim) != 0 || ve != 0) {
+  if constexpr (kExactV) {
+    // vlim is the largest scale that the unit ve takes
+    if (__ballot(vsm > vlim) != 0) {
+      float wm = 0.f;
+#pragma unroll
+      for (int i = 0; i < kWave; i += 16)
+        wm = fmaxf(wm, __builtin_bit_cast(float, __builtin_amdgcn_readlane(
+                                                     __builtin_bit_cast(int, vsm), i)));
+      int x = 5;
+      if (__builtin_isfinite(wm)) frexpf(wm, &x);
+      e = max(ve, min(max(__builtin_amdgcn_readfirstlane(x) - 5, kNoUnit), -kNoUnit));
+    }
+    e += kUnitBias;
+    if ((lane & 15) == 0) *reinterpret_cast<float4_t*>(&L.vs[buf][16 * w + 4 * (lane >> 4)]) = b.vs;
+  } else if (__ballot(vsm > vlim) != 0 || ve != 0) {
     if (__ballot(vsm > vlim) != 0) {
       float wm = 0.f;  // each group of 16 lanes holds the same scales
 #pragma unroll
@@ -499,6 +525,10 @@ __device__ __forceinline__ void convert_raw(const AttnArgs& a, const RawBlock<D>
       case 1: v = v_operand<1, KF>(col); break;
       case 2: v = v_operand<2, KF>(col); break;
       default: v = v_operand<3, KF>(col); break;
+    }
+    if constexpr (kExactV) {
+      vd[2 * (i % Lds::kRowsN * kWave + i / Lds::kRowsN)] = __builtin_bit_cast(uint2, v);
+      continue;
     }
     if constexpr (KF == kE5M2) {
       constexpr _Float16 down = (_Float16)(1.f / 256.f);
@@ -565,7 +595,7 @@ __device__ __forceinline__ void prefill_half(const PrefillLds<D>& L, int buf, in
                                              const QOp<QT, D> (&qop)[NT], const float (&back)[NT],
                                              const int (&lo)[NT], const int (&hi)[NT], int sinks,
                                              int lane,
-                                             bool vmix, half2_t vf,
+                                             bool vmix, half2_t vf, float vunit,
                                              float16v_t (&acc)[NT][D / 32], float (&m)[NT],
                                              float (&l)[NT], bool& bad_score) {
   using Lds = PrefillLds<D>;
@@ -700,7 +730,32 @@ __device__ __forceinline__ void prefill_half(const PrefillLds<D>& L, int buf, in
   }
   // weights rounded to f16; the sums take the same rounded weights as the numerator
   typedef uint32_t word4_t __attribute__((ext_vector_type(4)));
-  word4_t pop[NT][2];
+  constexpr bool kExactV = exact_v<QT>();
+  constexpr int kPTerms = kExactV && sizeof(QT) == 4 ? 2 : 1;
+  word4_t pop[NT][2], pop2[kPTerms == 2 ? NT : 1][2];
+  if constexpr (kExactV) {
+    // times the V scales in the unit, then rounded; the sums take the weights as they are
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const float4_t vs = *reinterpret_cast<const float4_t*>(&L.vs[buf][32 * kt + 8 * x + 4 * h]) * vunit;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int y = 0; y < 4; y += 2) {
+          const float p0 = __builtin_amdgcn_exp2f(s[t][4 * x + y]);
+          const float p1 = __builtin_amdgcn_exp2f(s[t][4 * x + y + 1]);
+          l[t] += p0 + p1;
+          float w0 = p0 * vs[y], w1 = p1 * vs[y + 1];
+          if constexpr (kPTerms == 2) asm volatile("" : "+v"(w0), "+v"(w1));  // one value for both terms
+          const uint32_t pair = pack2<_Float16>(w0, w1);
+          pop[t][x / 2][2 * (x % 2) + y / 2] = pair;
+          if constexpr (kPTerms == 2) {
+            const half2_t hi = __builtin_bit_cast(half2_t, pair);
+            pop2[t][x / 2][2 * (x % 2) + y / 2] = pack2<_Float16>(w0 - (float)hi[0], w1 - (float)hi[1]);
+          }
+        }
+    }
+  } else
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -748,6 +803,12 @@ __device__ __forceinline__ void prefill_half(const PrefillLds<D>& L, int buf, in
       for (int t = 0; t < NT; ++t)
         acc[t][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
             vop[x], __builtin_bit_cast(half8_t, pop[t][w]), acc[t][n], 0, 0, 0);
+      if constexpr (kPTerms == 2) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+          acc[t][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+              vop[x], __builtin_bit_cast(half8_t, pop2[t][w]), acc[t][n], 0, 0, 0);
+      }
     }
 }
 
@@ -878,8 +939,11 @@ __device__ __forceinline__ void prefill_unit(const AttnArgs& a, PrefillLds<D>& L
   }
   // The PV accumulators are in units of 2^-ve: ve is the largest block exponent so far
   // (0 unless a block's V scales need more, see convert_raw); vlim is its scale limit.
-  int ve = 0;
-  float vlim = 32768.f / format_max<KF>();
+  // exact_v: the unit, kNoUnit before the first block, and the largest scale it takes.
+  constexpr bool kExactV = exact_v<QT>();
+  int ve = kExactV ? kNoUnit : 0;
+  float vlim = kExactV ? -1.f : 32768.f / format_max<KF>();
+  float vunit = 1.f;
 
   // steps [inner_lo, inner_hi) see every key of theirs with every valid column
   const int keys0 = b_lo * kBlockTokens;
@@ -889,7 +953,7 @@ __device__ __forceinline__ void prefill_unit(const AttnArgs& a, PrefillLds<D>& L
   const int inner_hi = wb.any && inner_end > 0 ? inner_end / kStepKeys : 0;
   if (nsteps > 0) {
     if constexpr (!QOp<QT, D>::kAhead) load_step(0);
-    convert_raw<D, QOp<QT, D>::kPad>(a, raw, L, 0, wave, lane, masks, ve, vlim);
+    convert_raw<D, QOp<QT, D>::kPad, exact_v<QT>()>(a, raw, L, 0, wave, lane, masks, ve, vlim);
     if (nsteps > 1) load_step(1);
     __syncthreads();
   }
@@ -906,7 +970,21 @@ __device__ __forceinline__ void prefill_unit(const AttnArgs& a, PrefillLds<D>& L
     bool vmix = false;
     uint32_t slow = scaled ? kScaledBit : 0u;
     half4_t vf = {(_Float16)1.f, (_Float16)1.f, (_Float16)1.f, (_Float16)1.f};
-    if (__builtin_expect((f0 | f1 | f2 | f3 | ve) != 0, 0)) {
+    if constexpr (kExactV) {
+      if (((f0 | f1 | f2 | f3) & kLargeFlag) != 0) slow = kScaledBit | kLargeBit;
+      constexpr int kMask = kLargeFlag - 1;
+      const int emax = max(max(f0 & kMask, f1 & kMask), max(f2 & kMask, f3 & kMask)) - kUnitBias;
+      if (__builtin_expect(emax > ve || vlim < 0.f, 0)) {
+        const float down = ldexpf(1.f, ve - emax);  // (0 accumulators before the first)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int n = 0; n < kRowsN; ++n) acc[t][n] *= down;
+        ve = emax;
+        vlim = ldexpf(1.f, ve + 7);
+        vunit = ldexpf(1.f, -ve);
+      }
+    } else if (__builtin_expect((f0 | f1 | f2 | f3 | ve) != 0, 0)) {
       if (((f0 | f1 | f2 | f3) & kLargeFlag) != 0) slow = kScaledBit | kLargeBit;
       const int e4[kWaves] = {f0 & (kLargeFlag - 1), f1 & (kLargeFlag - 1), f2 & (kLargeFlag - 1),
                               f3 & (kLargeFlag - 1)};
@@ -947,22 +1025,22 @@ __device__ __forceinline__ void prefill_unit(const AttnArgs& a, PrefillLds<D>& L
       if (mine != 0)
         prefill_half<QT, D, NT>(L, buf, half, mine | slow, bounded >> (2 * half) & 3u, masks,
                                 kb0 + 32 * half, kop, []() {}, qop, back, lo, hi, sink.keys, lane, vmix,
-                                half != 0 ? half2_t{vf[2], vf[3]} : half2_t{vf[0], vf[1]}, acc, m,
-                                l, bad_score);
+                                half != 0 ? half2_t{vf[2], vf[3]} : half2_t{vf[0], vf[1]}, vunit, acc,
+                                m, l, bad_score);
     } else if (use != 0) {
       prefill_half<QT, D, NT>(L, buf, 0, (use & 3u) | slow, bounded & 3u, masks, kb0, kop,
                               [&]() __attribute__((always_inline)) {
                                 load_k_operands<D>(L, buf, 1, lane, kop);
                               },
-                              qop, back, lo, hi, sink.keys, lane, vmix, half2_t{vf[0], vf[1]}, acc, m,
+                              qop, back, lo, hi, sink.keys, lane, vmix, half2_t{vf[0], vf[1]}, vunit, acc, m,
                               l, bad_score);
       prefill_half<QT, D, NT>(L, buf, 1, use >> 2 | slow, bounded >> 2, masks, kb0 + 32, kop,
-                              []() {}, qop, back, lo, hi, sink.keys, lane, vmix, half2_t{vf[2], vf[3]}, acc,
+                              []() {}, qop, back, lo, hi, sink.keys, lane, vmix, half2_t{vf[2], vf[3]}, vunit, acc,
                               m, l, bad_score);
     }
     if (i + 1 < nsteps) {
       // the other buffer was last read in step i - 1, before the barrier that ended it
-      convert_raw<D, QOp<QT, D>::kPad>(a, raw, L, buf ^ 1, wave, lane, masks, ve, vlim);
+      convert_raw<D, QOp<QT, D>::kPad, exact_v<QT>()>(a, raw, L, buf ^ 1, wave, lane, masks, ve, vlim);
       if (i + 2 < nsteps) load_step(i + 2);
     }
     __syncthreads();
@@ -1012,7 +1090,8 @@ __device__ __forceinline__ void prefill_unit(const AttnArgs& a, PrefillLds<D>& L
     // that it is the same value)
     int f = (group * NT + t) * 32 + (lane_id() & 31);
     asm volatile("" : "+v"(f));
-    store(t, acc[t], m[t], sum32(l[t]), ve, column_of(f));
+    // (E4M3FN codes enter as 2^-8 of their values)
+    store(t, acc[t], m[t], sum32(l[t]), kExactV && KF == kE4M3 ? ve + 8 : ve, column_of(f));
   }
   mark(5);
 }
