@@ -79,6 +79,13 @@ class KeyWeights:
             raise ValueError(f"{what} must have one row per sequence")
 
 
+def check_budget(keep, recent, sinks):
+    """The tokens an eviction keeps, and those of them that stay for their place."""
+    if any(type(v) is not int or v < 0 for v in (keep, recent, sinks)) or keep < 1 \
+            or sinks + recent > keep:
+        raise ValueError("keep must be a positive int that holds the sinks and recent tokens")
+
+
 def require_rows(cache, selected, num_seqs, what="key_weights"):
     if not isinstance(selected, KeyWeightRows):
         raise ValueError(f"{what} must be rows selected from a KeyWeights")

@@ -48,6 +48,8 @@ class _PagedSnapshot:
     scales: torch.Tensor  # host fp32 [P, L, 2, Hkv, bs]
     valid: torch.Tensor   # host uint8 [P, bs]: the pages' padding leaves (0 = padding key)
     nbytes: int
+    evicted: int = 0      # the sequence's evictions (PagedSequence.evicted, floor)
+    floor: int = 0
 
 
 class _Catalog:
@@ -187,15 +189,17 @@ class PagedStateArchive:
                 self._catalog.refund(nbytes)
                 raise
         return self._catalog.file(_PagedSnapshot(sequence.identity, length, codes, scales,
-                                                 valid, nbytes))
+                                                 valid, nbytes, sequence.evicted,
+                                                 sequence.floor))
 
     def restore(self, handle, *, identity):
         """Fresh pages holding the archived tokens, as a new sequence of ``identity``;
         the snapshot stays archived until ``release``."""
         snapshot = self._catalog.lookup(handle, identity)
+        past = {"evicted": snapshot.evicted, "floor": snapshot.floor} if snapshot.floor else {}
         sequence = self.pool.restore_pages((snapshot.codes, snapshot.scales, snapshot.valid),
                                            identity=identity, length=snapshot.length,
-                                           stream=self._copy_stream())
+                                           stream=self._copy_stream(), **past)
         self._catalog.note_restored(snapshot.length)
         return sequence
 

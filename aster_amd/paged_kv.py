@@ -35,7 +35,7 @@ import torch
 
 from . import _native
 from .attention_backend import BACKEND, KernelWork, UnsupportedAttentionBackend
-from .key_weights import EvictedTokens, require_rows
+from .key_weights import EvictedTokens, check_budget, require_rows
 from .kv_quantization import KVQuantization, QuantizedKV, _DTYPE_CODES, require_format
 
 DEFAULT_PARTITION_TOKENS = 0  # automatic: stream-K for bf16/fp16, else 512-token partitions
@@ -645,8 +645,7 @@ class PagedKVCache:
         if context_lens.shape[0] != num_seqs:
             raise ValueError("block_tables/context_lens must have one row per sequence")
         weights = require_rows(self, key_weights, num_seqs)
-        if any(type(v) is not int or v < 0 for v in (keep, recent, sinks)) or keep < 1                 or sinks + recent > keep:
-            raise ValueError("keep must be a positive int that holds the sinks and recent tokens")
+        check_budget(keep, recent, sinks)
         if max_context_len > block_tables.shape[1] * self.block_size:
             raise ValueError("max_context_len exceeds the block table capacity")
         if max_context_len > weights.capacity:

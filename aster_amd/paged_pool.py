@@ -39,6 +39,7 @@ import numpy as np
 import torch
 
 from .attention_backend import UnsupportedAttentionBackend
+from .key_weights import check_budget, require_rows
 from .kv_quantization import KVQuantization, QuantizedKV, require_format
 
 
@@ -91,6 +92,10 @@ class PagedSequence:
     pages: list = field(default_factory=list)
     length: int = 0
     released: bool = False
+    # tokens evicted so far (the next token's position is length + evicted), and the length an
+    # eviction left: below it the KV heads hold different tokens
+    evicted: int = 0
+    floor: int = 0
 
 
 @dataclass(frozen=True)
@@ -263,17 +268,90 @@ class PagedStatePool:
             for ref in sequence.pages:
                 self._page(ref).owners += 1
             return PagedSequence(id(self), sequence.kind, sequence.identity, list(sequence.pages),
-                                 sequence.length)
+                                 sequence.length, evicted=sequence.evicted, floor=sequence.floor)
 
     def truncate(self, sequence, length):
         with self._lock:
             self._check(sequence)
             if not 0 <= length <= sequence.length:
                 raise ValueError("Cannot extend state by truncation")
+            if 0 < length < sequence.floor:
+                raise ValueError("Cannot truncate into the tokens an eviction left")
+            if length == 0:
+                sequence.evicted = sequence.floor = 0
             count = math.ceil(length / self.block_size)
             self._drop(sequence.pages[count:])
             sequence.pages = sequence.pages[:count]
             sequence.length = length
+
+    def evict(self, sequences, key_weights, *, keep, recent=0, sinks=0):
+        """Cut ``sequences`` (distinct) to ``keep`` tokens each, per layer and KV head those
+        that gathered the most weight (``PagedKVCache.evict``; ``key_weights``: their rows, in
+        the same order, of which the first ``length`` weights are read). Sequences of no more
+        tokens are left as they are (padding tokens leave in any case). Pages that no other
+        sequence or reader holds are compacted in place; of others the tokens move to fresh
+        pages, and the sequence lets go of the shared ones (``CacheCapacityError`` if there
+        are too few, nothing changed). Waits for the device; returns the new lengths.
+
+        The dropped tokens count in ``sequence.evicted``: positions go on behind them, and the
+        sequence cannot be truncated into the tokens that stayed. No reference counterpart
+        (state.py keeps every token)."""
+        sequences = list(sequences)
+        if not sequences or len({id(s) for s in sequences}) != len(sequences):
+            raise ValueError("Eviction takes a nonempty batch of distinct sequences")
+        with self._lock:
+            for s in sequences:
+                self._check(s)
+            cache = self.cache
+            if cache is None:
+                raise StateError("The pool's arena is not allocated before its first append")
+            weights = require_rows(cache, key_weights, len(sequences))
+            check_budget(keep, recent, sinks)
+            todo = [i for i, s in enumerate(sequences)
+                    if s.length > keep or (cache.has_padding and s.length)]
+            shared = [i for i in todo if any(self._page(ref).owners > 1 or self._page(ref).readers
+                                             for ref in sequences[i].pages)]
+            own = [i for i in todo if i not in set(shared)]
+            most = [math.ceil(min(keep, sequences[i].length) / self.block_size) for i in shared]
+            fresh = self._allocate(sum(most))
+            try:
+                took, at, lengths = {}, 0, {}
+                for i, n in zip(shared, most):
+                    took[i], at = fresh[at:at + n], at + n
+                for group in (shared, own):
+                    if not group:
+                        continue
+                    rows = [sequences[i] for i in group]
+                    longest = max(s.length for s in rows)
+                    got = cache.evict(
+                        self._table([s.pages for s in rows]),
+                        torch.tensor([s.length for s in rows], dtype=torch.int32).to(cache.device),
+                        weights.select([key_weights.rows[i] for i in group]), keep=keep,
+                        recent=recent, sinks=sinks, max_context_len=longest,
+                        dst_tables=self._table([took[i] for i in group]) if group is shared else None)
+                    lengths.update(zip(group, got.lengths.tolist()))
+                cache.raise_errors()
+            except BaseException:
+                self._drop(fresh)
+                raise
+            for i in todo:
+                s, length = sequences[i], lengths[i]
+                pages = took.get(i, s.pages)
+                count = math.ceil(length / self.block_size)
+                self._drop(pages[count:] if i not in took else s.pages + pages[count:])
+                for index, ref in enumerate(pages[:count]):
+                    page = self._page(ref)
+                    page.valid = max(page.valid, min(self.block_size, length - index * self.block_size))
+                s.evicted += s.length - length
+                s.pages, s.length, s.floor = list(pages[:count]), length, length
+            return tuple(s.length for s in sequences)
+
+    def _table(self, rows):
+        """A device block table of pages per row (entries past a row's are 0)."""
+        table = np.zeros((len(rows), max([len(r) for r in rows] + [1])), dtype=np.int32)
+        for i, refs in enumerate(rows):
+            table[i, :len(refs)] = [ref.index for ref in refs]
+        return torch.from_numpy(table).to(self.cache.device)
 
     def release(self, sequence):
         with self._lock:
@@ -600,7 +678,7 @@ class PagedStatePool:
             blocks = [ref.index for ref in sequence.pages]
         return self.cache.gather_blocks(blocks, stream=stream)
 
-    def restore_pages(self, payloads, *, identity, length, stream=None):
+    def restore_pages(self, payloads, *, identity, length, stream=None, evicted=0, floor=0):
         """Reserve every destination page, move the archived codes and scales in
         without requantization, publish after the copy completes (state.py:427-493).
 
@@ -609,8 +687,10 @@ class PagedStatePool:
         ``[1, Hkv, count, 1]`` fp32 scales, optionally followed by the padding leaf
         ``[1, 1, count, 1]`` (what ``read_pages`` exposes and ``PagedStateArchive``
         keeps), or ``(codes, scales[, valid])`` already packed in the
-        ``export_blocks`` layout on the host."""
+        ``export_blocks`` layout on the host. ``evicted``, ``floor``: the archived
+        sequence's."""
         sequence = self.create(identity)
+        sequence.evicted, sequence.floor = evicted, floor
         if type(length) is not int or length < 1:
             raise StateError("Archived page count and token length differ")
         if self.cache is None:  # no arena yet: its layout is unknown (state.py:453-454)

@@ -34,6 +34,7 @@ import numpy as np
 import torch
 
 from .attention_backend import BACKEND, KernelWork, UnsupportedAttentionBackend
+from .key_weights import require_rows
 from .kv_quantization import KVQuantization
 from .paged_pool import KVStateCodec, PagedStatePool, StateError
 from .prefix_plan import plan_prefix_packs
@@ -88,10 +89,14 @@ def _padding_vector(padding, counts):
 
 
 class PagedAttentionStep:
-    """One step of ``counts[b]`` new tokens for each sequence ``b`` of a batch."""
+    """One step of ``counts[b]`` new tokens for each sequence ``b`` of a batch. With
+    ``key_weights`` (the sequences' rows, ``KeyWeights.select``) every layer's attention
+    gathers its keys' weights for ``PagedStatePool.evict``; what an aborted step gathered
+    stays gathered, but for its own tokens. ``positions``: the rows' first new positions,
+    tokens evicted before counted."""
 
     def __init__(self, pool, sequences, counts, *, padding=None, work=None,
-                 partition_tokens=0):
+                 partition_tokens=0, key_weights=None):
         if not sequences or len(sequences) != len(counts) or \
                 len({id(s) for s in sequences}) != len(sequences):
             raise ValueError("Need a nonempty batch of distinct sequences and aligned chunks")
@@ -103,6 +108,8 @@ class PagedAttentionStep:
         self.pool, self.counts = pool, list(counts)
         self.work = work if work is not None else KernelWork()
         self.partition_tokens = partition_tokens
+        self.key_weights = key_weights
+        self.evicted = [s.evicted for s in sequences]
         self.reservations = []
         self._tables = None
         self._open = False
@@ -120,9 +127,13 @@ class PagedAttentionStep:
                 starts.append(starts[-1] + n)
             self.num_tokens = starts[-1]
             self.query_start_loc = _device_ints(starts, torch.int32, device)
-            self.positions = [r.start for r in self.reservations]
+            self.positions = [r.start + n for r, n in zip(self.reservations, self.evicted)]
             self.max_query_len = max(counts)
             self.max_context_len = max(r.length for r in self.reservations)
+            if key_weights is not None:
+                weights = require_rows(cache, key_weights, len(counts))
+                if weights.capacity < self.max_context_len:
+                    raise ValueError("the step exceeds the key weights' capacity")
             slots = [s for r in self.reservations for s in r.slots]
             self.slot_mapping = _device_ints(slots, torch.int64, device)
             cache.write_key_valid(self.slot_mapping,
@@ -141,17 +152,33 @@ class PagedAttentionStep:
             raise
         self._open = True
 
-    def attend(self, layer, query, key, value, *, scale=None, window=None, out=None):
+    def attend(self, layer, query, key, value, *, scale=None, window=None, out=None, sinks=None):
         """Append this layer's chunk K/V and attend. ``query`` ``[T, Hq, D]`` and
         ``key``/``value`` ``[T, Hkv, D]`` packed by row in batch order (``pack_rows``
         converts the reference's ``[B, H, Q, D]``). Returns ``[T, Hq, D]`` in the
-        query dtype."""
+        query dtype. ``sinks``: the first tokens that stay visible beside ``window``."""
         if not self._open:
             raise StateError("Step already committed or aborted")
         if query.shape[0] != self.num_tokens or key.shape[0] != self.num_tokens:
             raise ValueError("query/key rows must match the step's tokens")
         cache = self.pool.cache
         ws_work = self.work
+        if window is not None and any(self.evicted):
+            raise UnsupportedAttentionBackend("windows count positions, which a sequence with "
+                                              "evicted tokens no longer has")
+        if window is not None and self.key_weights is not None:
+            raise UnsupportedAttentionBackend("key weights are gathered over all keys, not a window")
+        if self.key_weights is not None or sinks is not None:
+            cache.append(layer, key, value, self.slot_mapping, reserved=True)
+            chunks = self.max_query_len > 1
+            common = dict(max_context_len=self.max_context_len, scale=scale, out=out, work=ws_work,
+                          query_start_loc=self.query_start_loc if chunks else None,
+                          max_query_len=self.max_query_len if chunks else None)
+            if self.key_weights is not None:
+                return cache.paged_attention_weights(layer, query, self.block_tables,
+                                                     self.context_lens, self.key_weights, **common)
+            return cache.paged_attention(layer, query, self.block_tables, self.context_lens,
+                                         window=window, sinks=sinks, **common)
         plan = self._decode_plan(query, window) if self.partition_tokens == 0 else None
         if plan is not None:
             # decode rows on the host schedule (one per step and shape); rows aliasing
@@ -354,12 +381,15 @@ def _synchronize(device):
 
 
 def hip_forward(runner, sequences, chunks, *, return_all_logits=False, padding_masks=None,
-                hidden_state_indices=None):
+                hidden_state_indices=None, key_weights=None):
     """``PagedAttentionRunner.forward_batch`` (paged_attention.py:110-230) on a runner set
     up by :func:`bind_hip_backend`: the reference's argument checks and model walk, with
     every layer's attention as one ``PagedAttentionStep`` launch pair. With
     ``hidden_state_indices`` (see :func:`hip_forward_features`) every row's result is
-    ``(logits, features)``."""
+    ``(logits, features)``. ``key_weights``: the sequences' rows, for models without
+    windows, to gather their keys' weights (``PagedAttentionStep``). A layer whose
+    ``self_attn`` has ``sink_tokens`` beside its ``window`` keeps that many first tokens
+    visible."""
     if not sequences or len(sequences) != len(chunks) or \
             len({id(value) for value in sequences}) != len(sequences):
         raise ValueError("Need a nonempty batch of distinct sequences and aligned chunks")
@@ -371,13 +401,16 @@ def hip_forward(runner, sequences, chunks, *, return_all_logits=False, padding_m
     model = runner.model
     config = model.config
     start, count, batch = next(iter(starts)), next(iter(counts)), len(sequences)
-    if start + count > config.max_position_embeddings:
+    evicted = [s.evicted for s in sequences]
+    if start + max(evicted) + count > config.max_position_embeddings:
         raise ValueError("Sequence exceeds declared position support")
     if any(type(t) is not int or not 0 <= t < config.vocab_size for c in chunks for t in c):
         raise ValueError("Input token outside this immutable model vocabulary")
     device = runner.device
     ids = torch.tensor(chunks, device=device, dtype=torch.long)
     positions = torch.arange(start, start + count, device=device).expand(batch, -1)
+    if any(evicted):
+        positions = positions + torch.tensor(evicted, device=device)[:, None]
     padding = None
     if padding_masks is not None:
         padding = torch.as_tensor(padding_masks).cpu()
@@ -391,7 +424,8 @@ def hip_forward(runner, sequences, chunks, *, return_all_logits=False, padding_m
     with torch.inference_mode():
         step = PagedAttentionStep(pool, sequences, [count] * batch, padding=padding,
                                   work=runner.attention_work,
-                                  partition_tokens=runner.partition_tokens)
+                                  partition_tokens=runner.partition_tokens,
+                                  key_weights=key_weights)
         try:
             _synchronize(device)
             started = time.monotonic()
@@ -416,7 +450,8 @@ def hip_forward(runner, sequences, chunks, *, return_all_logits=False, padding_m
                         pool._lock_signature((runner.num_layers, runner.num_kv_heads,
                                               runner.head_dim, key.dtype))
                 attended = step.attend(index, _packed(query), _packed(key), _packed(value),
-                                       scale=attention.scale, window=attention.window)
+                                       scale=attention.scale, window=attention.window,
+                                       sinks=getattr(attention, "sink_tokens", None) or None)
                 hidden = hidden + attention.o_proj(attended.reshape(batch, count, -1))
                 hidden = hidden + layer.mlp(layer.post_attention_layernorm(hidden))
             normed = model.model.norm(hidden)
@@ -498,9 +533,10 @@ class PagedAttentionRunner:
         return cls(loader(artifact.path), policy_artifact_id=artifact.id, tokenizer=tokenizer,
                    **kwargs)
 
-    def forward_batch(self, sequences, chunks, *, return_all_logits=False, padding_masks=None):
+    def forward_batch(self, sequences, chunks, *, return_all_logits=False, padding_masks=None,
+                      key_weights=None):
         return hip_forward(self, sequences, chunks, return_all_logits=return_all_logits,
-                           padding_masks=padding_masks)
+                           padding_masks=padding_masks, key_weights=key_weights)
 
     def forward_feature_batch(self, sequences, chunks, *, hidden_state_indices):
         return hip_forward_features(self, sequences, chunks,
