@@ -75,11 +75,13 @@ Plan plan_call(const Shape& s) {
   // every CU takes several units (128 rows, window 4096: 164 us a call against 167 with 8 waves and
   // 174 with 4), 8 where it takes one or none (48 rows, 4 KV heads, window 1024: 15.3 against
   // 17.8 and 20.2).
-  p.waves = units <= cus ? 8 : wide_waves(s.head_dim);
+  // Long rows of few units are cut into pieces in any case, which four waves balance better (16
+  // rows of 32768 keys with their weights, groups of 8: 291 us against 309 with 8).
+  p.waves = units > cus ? wide_waves(s.head_dim, s.weights && s.terms == 2) : units * blocks >= 256 * cus ? 4 : 8;
   // pieces: of 64 blocks a wave at most, and enough of them to give every CU 16 waves
   int64_t parts = (blocks + (int64_t)p.waves * kIdsPerWave - 1) / ((int64_t)p.waves * kIdsPerWave);
   const int64_t want = 16 * cus / (units * p.waves);
-  const int64_t most = blocks / (4 * p.waves);  // (four blocks a wave are worth a piece)
+  const int64_t most = blocks / (8 * p.waves);  // (eight blocks a wave are worth a launch more)
   parts = std::max(parts, std::min(want, most));
   parts = std::max<int64_t>(parts, 1);
   p.part_blocks = (int32_t)((blocks + parts - 1) / parts);
@@ -257,6 +259,9 @@ int bounded_attention(const Call& c) {
   a.part_blocks = plan.part_blocks;
   a.max_parts = plan.parts;
   a.total_waves = plan.waves;
+  // (rows of one sliding window are about equally long; one workgroup a CU or less starts at once)
+  const int64_t units = (int64_t)c.num_seqs * cache->num_kv_heads;
+  a.longest_first = w != nullptr && c.num_seqs <= 128 && units > device_cus() && units <= 4 * device_cus();
   char* ws = static_cast<char*>(c.workspace);
   a.ws_o = reinterpret_cast<float*>(ws);
   a.ws_ml = reinterpret_cast<float*>(ws + plan.o_bytes);

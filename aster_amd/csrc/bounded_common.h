@@ -21,6 +21,7 @@ struct BoundedArgs : AttnArgs {
   int32_t sinks;        // keys [0, sinks) stay visible beside the window
   int32_t max_context;  // host bound of context_lens
   int32_t group;        // query heads per KV head
+  int32_t longest_first;  // decode with key weights: rows in the order of their lengths
   // decode: a row's visible blocks in pieces of part_blocks (AttnArgs), at most max_parts
   KeyWeights kw;
   // base-2 scores of every key, [num_seqs * num_kv_heads * group][score_stride]; weights only
@@ -110,8 +111,11 @@ ASTR_BY_FORMAT(launch_chunk_weights, BoundedArgs)
 ASTR_BY_FORMAT(launch_prefill_sinks, SinkChunkArgs)
 #undef ASTR_BY_FORMAT
 
-// Waves of the decode kernel's workgroup: four, or as many as the LDS holds stages for.
-constexpr int wide_waves(int head_dim) { return head_dim == 256 ? 8 : 16; }
+// Waves of the decode kernel's widest workgroup: as many as the LDS holds stages for, and the
+// registers (fp32 queries with key weights do not fit the 128 of 16 waves).
+constexpr int wide_waves(int head_dim, bool fp32_weights) {
+  return head_dim == 256 || fp32_weights ? 8 : 16;
+}
 
 }  // namespace attn
 }  // namespace astr

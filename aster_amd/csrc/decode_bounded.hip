@@ -18,7 +18,7 @@
 // bits of the query), FP8 codes an f16 query; softmax weights enter the output's products
 // rounded to f16, the sums in fp32 before that rounding. fp32 queries: FP8 codes meet two
 // f16 terms of the query, and the weights enter as two f16 terms (22 bits).
-#include <type_traits>
+#include <climits>
 
 #include "bounded_common.h"
 
@@ -118,15 +118,13 @@ struct VUnit {
 };
 
 // One staged block through the MFMAs. Lane (qg, r) holds the scores of keys 4 qg + j for
-// head r; raw scores of keys outside [lo, hi) and of padding keys are -inf. `scores` (WEIGHTS):
-// where the lane's four scores go.
-template <typename QT, int D, bool WEIGHTS>
-__device__ __forceinline__ void bounded_block(const char* st,
+// head r; those of keys outside [lo, hi) and of padding keys are -inf. Returns them.
+template <typename QT, int D>
+__device__ __forceinline__ float4_t bounded_block(const char* st,
                                               const int4_t (&q)[SharedQuery<QT, D>::kOps],
                                               float cf, int tok_base, int lo, int hi, bool gvalid, int r,
                                               int qg, float4_t (&acc)[D / 16], float& m, float& l,
-                                              VUnit& vu, bool& bad_score, bool masks,
-                                              float* scores) {
+                                              VUnit& vu, bool& bad_score, bool masks) {
   using S = Stage<D>;
   using Q = SharedQuery<QT, D>;
   constexpr int KCH = D / 64, VB = D / 16, NPV = D / 16;
@@ -215,9 +213,6 @@ __device__ __forceinline__ void bounded_block(const char* st,
     for (int n = 0; n < NPV; ++n) acc[n] *= alpha;
     m = mn;
   }
-  if constexpr (WEIGHTS) {
-    if (gvalid) *reinterpret_cast<float4_t*>(scores) = float4_t{sc[0], sc[1], sc[2], sc[3]};
-  }
   constexpr int kTerms = sizeof(QT) == 4 ? 2 : 1;
   half4_t pop[kTerms];
 #pragma unroll
@@ -257,6 +252,7 @@ __device__ __forceinline__ void bounded_block(const char* st,
     for (int t = 0; t < kTerms; ++t)
       acc[n] = __builtin_amdgcn_mfma_f32_16x16x16f16(vop, pop[t], acc[n], 0, 0, 0);
   }
+  return float4_t{sc[0], sc[1], sc[2], sc[3]};
 }
 
 // Adds the weights of keys [t0, t1) of one (sequence, KV head): its scores (base 2) at
@@ -297,6 +293,32 @@ __device__ __forceinline__ float log_sum(float m, float l) {
   return l > 0.f ? m + __builtin_amdgcn_logf(l) : INFINITY;
 }
 
+// The row that is `nth` by length, the longest first (of equal ones the lowest): a grid that deals
+// out few workgroups per CU then does not end on a long row alone (64 rows of 128 to 4096 tokens,
+// 8 KV heads, bf16: 85 us instead of 90). At most kOrderRows rows; every thread calls it.
+constexpr int kOrderRows = 128;
+__device__ __forceinline__ int nth_longest(const BoundedArgs& a, int nth, char* lds) {
+  int* const len = reinterpret_cast<int*>(lds);  // kOrderRows lengths, then the row
+  const int t = threadIdx.x;
+  if (t < kOrderRows) len[t] = t < a.num_seqs ? a.context_lens[t] : INT_MIN;
+  __syncthreads();
+  if (t < a.num_seqs) {
+    const int mine = len[t];
+    int rank = 0;
+#pragma unroll 1
+    for (int j = 0; j < a.num_seqs; j += 4) {
+      const int4_t v = *reinterpret_cast<const int4_t*>(len + j);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) rank += v[i] > mine || (v[i] == mine && j + i < t);
+    }
+    if (rank == nth) len[kOrderRows] = t;
+  }
+  __syncthreads();
+  const int seq = __builtin_amdgcn_readfirstlane(len[kOrderRows]);
+  __syncthreads();  // the stages take the lengths' place
+  return seq;
+}
+
 template <int D, int NW>
 struct BoundedLds {
   static constexpr int kStageBytes = NW * Stage<D>::kBytes;
@@ -320,10 +342,11 @@ __global__ __launch_bounds__(NW * kWave) void bounded_decode_kernel(BoundedArgs 
   __shared__ SharedQuery<QT, D> query;
   __shared__ float lse[16];
 
-  const int part = blockIdx.x, kvh = blockIdx.y, seq = blockIdx.z;
+  const int part = blockIdx.x, kvh = blockIdx.y;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave;
   const int r = lane & 15, qg = lane >> 4;
+  const int seq = WEIGHTS && a.longest_first ? nth_longest(a, blockIdx.z, lds) : blockIdx.z;
   const int G = a.group;
   const bool gvalid = r < G;
   const int tok = decode_token(a, seq);
@@ -381,15 +404,22 @@ __global__ __launch_bounds__(NW * kWave) void bounded_decode_kernel(BoundedArgs 
   float* const srow = WEIGHTS ? a.scores + (unit * G + (gvalid ? r : 0)) * a.score_stride : nullptr;
 
   auto step = [&](int i, char* st) __attribute__((always_inline)) {
-    // block i has landed once only the next one's loads may be on their way (loads complete in
-    // order; a padding load or a score store among the younger ones makes this wait longer)
-    if (i + 1 < nblk) wait_vmcnt<S::kLoads>();
-    else wait_vmcnt<0>();
+    // block i has landed once only the next one's loads may be on their way, and (WEIGHTS) the
+    // score store issued after them: vector-memory operations complete in order (a padding load
+    // among the younger ones makes this wait longer). Stores ahead of the next loads instead made
+    // every block wait for the one before's (16 rows of 32768 tokens, 64 heads: 269 us, now 266).
+    if (i + 1 >= nblk) wait_vmcnt<0>();
+    else if (WEIGHTS && i > 0) wait_vmcnt<S::kLoads + 1>();
+    else wait_vmcnt<S::kLoads>();
     const int f = f0 + NW * i;
     const int base = v.block(f) * kBlockTokens;
-    bounded_block<QT, D, WEIGHTS>(st, q, cf, base, v.lo(f), v.hi(f), gvalid, r, qg, acc, m, l, vu,
-                                  bad_score, masks, WEIGHTS ? srow + base + 4 * qg : nullptr);
+    const float4_t sc = bounded_block<QT, D>(st, q, cf, base, v.lo(f), v.hi(f), gvalid, r, qg, acc, m, l,
+                                             vu, bad_score, masks);
     if (i + 2 < nblk) stage_block<D>(a, __builtin_amdgcn_readlane(ids, i + 2), kvh, lane, st);
+    if constexpr (WEIGHTS) {
+      asm volatile("" ::: "memory");  // the store stays behind the loads
+      if (gvalid) *reinterpret_cast<float4_t*>(srow + base + 4 * qg) = sc;
+    }
   };
   for (int i = 0; i < nblk; i += 2) {
     step(i, st0);
@@ -538,8 +568,11 @@ template <typename QT, int D>
 int launch_dim(const BoundedArgs& a, hipStream_t s) {
   const bool weights = a.kw.values != nullptr;
   // total_waves: the workgroup's waves
-  if constexpr (wide_waves(D) == 16) {
-    if (a.total_waves == 16) return weights ? launch<QT, D, 16, true>(a, s) : launch<QT, D, 16, false>(a, s);
+  if constexpr (wide_waves(D, sizeof(QT) == 4) == 16) {
+    if (a.total_waves == 16 && weights) return launch<QT, D, 16, true>(a, s);
+  }
+  if constexpr (wide_waves(D, false) == 16) {
+    if (a.total_waves == 16 && !weights) return launch<QT, D, 16, false>(a, s);
   }
   if (a.total_waves == 8) return weights ? launch<QT, D, 8, true>(a, s) : launch<QT, D, 8, false>(a, s);
   return weights ? launch<QT, D, 4, true>(a, s) : launch<QT, D, 4, false>(a, s);

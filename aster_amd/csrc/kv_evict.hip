@@ -146,10 +146,11 @@ __device__ __forceinline__ void find_digit(const int* hist, int need, int* wave_
 
 // Segments of up to R * T tokens: thread i holds the bits of tokens i, i + T, ... in registers,
 // read once; order comes from one prefix over the counts of all (round, wave) pairs.
-// Bound by the chain of barriers and LDS round trips of a segment, so that a CU holds as many
-// segments as it can: 256 threads up to 12288 tokens. 8 prompts of 1500 to 9000 tokens, 16 layers,
-// 8 heads: TIME_SELECT us; 58 with 1024 threads, 72 when every pass read the weights again and
-// every round of the last one waited for the one before.
+// Bound by the chain of barriers and LDS round trips of a segment and by its registers, of which
+// R a thread: the fewer threads, the cheaper a barrier, the fewer tokens a thread, the more
+// segments a CU holds. 8 prompts of 1500 to 9000 tokens, 16 layers, 8 heads: 40 us with 512 threads
+// (47 with 256, 57 with 1024; 58 with loads behind a branch per lane, 72 when every pass read the
+// weights again); the same prompts at 2200 to 4000 tokens: 22 us with 256 threads, 23 with 512.
 template <int T, int R>
 __global__ __launch_bounds__(T) void select_held_kernel(EvictArgs a) {
   constexpr int kWavesT = T / kWave, kPairs = R * kWavesT;
@@ -180,22 +181,47 @@ __global__ __launch_bounds__(T) void select_held_kernel(EvictArgs a) {
     if (sum && lane == 0) total = base;
   };
 
+  // Loads go out kBatch at a time, of clamped tokens and without a branch per lane: behind one,
+  // each waits for the load before it.
+  constexpr int kBatch = 8;
+  static_assert(R % kBatch == 0, "");
+  auto token = [&](int i) __attribute__((always_inline)) -> int { return min(i * T + (int)threadIdx.x, n - 1); };
   uint32_t u[R];  // 0: no token, or a padding one
 #pragma unroll
-  for (int i = 0; i < R; ++i) {
-    const int t = i * T + (int)threadIdx.x;
-    u[i] = t < n ? ordered(g.w[t]) : 0u;
+  for (int b = 0; b < R; b += kBatch) {
+    if (b * T < n) {  // (uniform, as every such test below)
+      float w[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) w[i] = g.w[token(b + i)];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) u[b + i] = (b + i) * T + (int)threadIdx.x < n ? ordered(w[i]) : 0u;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) u[b + i] = 0;
+    }
   }
   uint64_t fixed = 0;  // bit i: token i stays for its place
   int count = n;
   if (a.cache.key_valid != nullptr) {
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      if (i * T < n) {  // (uniform)
-        const int t = i * T + (int)threadIdx.x;
-        if (u[i] != 0 && !g.real(a, t)) u[i] = 0;
-        const uint64_t b = __ballot(u[i] != 0);
-        if (lane == 0) count_a[i * kWavesT + wave] = __builtin_popcountll(b);
+    for (int b = 0; b < R; b += kBatch) {
+      if (b * T < n) {
+        int id[kBatch];
+        uint8_t valid[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) id[i] = g.table[token(b + i) / kBlockTokens];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const bool in = (unsigned)id[i] < (unsigned)a.cache.num_blocks;
+          valid[i] = a.cache.key_valid[in ? (int64_t)id[i] * kBlockTokens + token(b + i) % kBlockTokens : 0];
+          valid[i] = in ? valid[i] : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          u[b + i] = valid[i] != 0 ? u[b + i] : 0u;
+          const uint64_t m = __ballot(u[b + i] != 0);
+          if (lane == 0 && (b + i) * T < n) count_a[(b + i) * kWavesT + wave] = __builtin_popcountll(m);
+        }
       }
     }
     __syncthreads();
@@ -207,7 +233,7 @@ __global__ __launch_bounds__(T) void select_held_kernel(EvictArgs a) {
       if (i * T < n) {
         const uint64_t b = __ballot(u[i] != 0);
         const int rank = count_a[i * kWavesT + wave] + lanes_below(b, lane);
-        if (u[i] != 0 && (rank < a.sinks || rank >= count - a.recent)) fixed |= 1ull << i;
+        fixed |= (uint64_t)(u[i] != 0 && (rank < a.sinks || rank >= count - a.recent)) << i;
       }
     }
     __syncthreads();  // count_a is written again
@@ -215,7 +241,7 @@ __global__ __launch_bounds__(T) void select_held_kernel(EvictArgs a) {
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const int t = i * T + (int)threadIdx.x;
-      if (t < n && (t < a.sinks || t >= n - a.recent)) fixed |= 1ull << i;
+      fixed |= (uint64_t)(t < n && (t < a.sinks || t >= n - a.recent)) << i;
     }
   }
   const int keep = min(a.keep, count);
@@ -278,15 +304,24 @@ __global__ __launch_bounds__(T) void select_held_kernel(EvictArgs a) {
   // stored (u becomes the weight's own bits)
   int at[R];
 #pragma unroll
-  for (int i = 0; i < R; ++i) {
-    at[i] = INT_MAX;
-    if (i * T < n) {
-      const bool more = more_of(i), tie = tie_of(i);
-      const uint64_t bm = __ballot(more), bt = __ballot(tie);
-      const int m = count_a[i * kWavesT + wave] + lanes_below(bm, lane);
-      const int e = count_b[i * kWavesT + wave] + lanes_below(bt, lane);
-      if (more || (tie && e < ties)) at[i] = m + min(e, ties);
-      if (at[i] < keep) u[i] = __builtin_bit_cast(uint32_t, g.w[i * T + (int)threadIdx.x]);
+  for (int b = 0; b < R; b += kBatch) {
+    if (b * T < n) {
+      float w[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) w[i] = g.w[token(b + i)];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const bool more = more_of(b + i), tie = tie_of(b + i);
+        const uint64_t bm = __ballot(more), bt = __ballot(tie);
+        const int pair = min((b + i) * kWavesT + wave, pairs - 1);  // (behind the pairs nothing stays)
+        const int m = count_a[pair] + lanes_below(bm, lane);
+        const int e = count_b[pair] + lanes_below(bt, lane);
+        at[b + i] = more || (tie && e < ties) ? m + min(e, ties) : INT_MAX;
+        u[b + i] = __builtin_bit_cast(uint32_t, w[i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) at[b + i] = INT_MAX;
     }
   }
   wait_vmcnt<0>();
@@ -611,8 +646,8 @@ extern "C" int astr_kv_evict(const astr_paged_kv* cache, int32_t num_layers,
     hipLaunchKernelGGL((select_held_kernel<256, 8>), segments, dim3(256), 0, s, a);
   else if (max_context_len <= 16 * 256)
     hipLaunchKernelGGL((select_held_kernel<256, 16>), segments, dim3(256), 0, s, a);
-  else if (max_context_len <= 48 * 256)
-    hipLaunchKernelGGL((select_held_kernel<256, 48>), segments, dim3(256), 0, s, a);
+  else if (max_context_len <= 24 * 512)
+    hipLaunchKernelGGL((select_held_kernel<512, 24>), segments, dim3(512), 0, s, a);
   else if (max_context_len <= 32 * kThreads)
     hipLaunchKernelGGL((select_held_kernel<kThreads, 32>), segments, dim3(kThreads), 0, s, a);
   else
