@@ -43,12 +43,11 @@ struct Shape {
 struct Plan {
   int32_t waves, part_blocks, parts;     // decode
   int64_t score_stride;
-  int32_t chunk_pieces, chunk_steps, column_pieces, column_tiles;  // chunks' weights
-  size_t o_bytes, ml_bytes, score_bytes, chunk_bytes, prefill_bytes;
+  int32_t column_pieces, column_tiles;   // chunks' weights
+  size_t o_bytes, ml_bytes, score_bytes, column_bytes, prefill_bytes;
   size_t decode() const { return o_bytes + ml_bytes + score_bytes; }
-  // the decode launches, the prefill launch and the chunks' weights follow one another on the
-  // stream and share the bytes
-  size_t total() const { return std::max(decode(), std::max(chunk_bytes, prefill_bytes)); }
+  // the decode launches and the chunks' follow one another on the stream and share the bytes
+  size_t total() const { return std::max(decode(), prefill_bytes + column_bytes); }
 };
 
 // Blocks of the longest row's visible list at most.
@@ -60,7 +59,7 @@ int64_t visible_blocks(const Shape& s) {
   return std::min(all + 1, seen);  // (a block of sinks and window keys is listed twice)
 }
 
-constexpr int64_t kMostPieces = 32;  // of a chunk's keys or columns
+constexpr int64_t kMostPieces = 32;  // of a chunk's columns
 
 // Partials of the prefill launch's split units: what a call of this shape may use.
 constexpr size_t kPrefillPartials = (size_t)64 << 20;
@@ -99,17 +98,7 @@ Plan plan_call(const Shape& s) {
     p.prefill_bytes = kPrefillPartials;
     if (s.weights) {
       const int64_t group = s.num_q_heads / s.num_kv_heads;
-      const int64_t ctiles = std::max<int64_t>(
-          std::min((int64_t)s.num_seqs * (((int64_t)s.max_q_len * group + 127) / 128),
-                   (int64_t)s.num_q_tokens * group / 128 + s.num_seqs) * s.num_kv_heads, 1);
-      const int64_t steps = (blocks + kWaves - 1) / kWaves;
-      // first pass: pieces of steps for eight workgroups a CU, of 8 steps at least (a prompt's
-      // early tokens see few keys, half of these workgroups have nothing to do)
-      int64_t per = std::max<int64_t>((ctiles * steps + 8 * cus - 1) / (8 * cus), 8);
-      per = std::max(per, (steps + kMostPieces - 1) / kMostPieces);
-      p.chunk_steps = (int32_t)std::min(per, steps);
-      p.chunk_pieces = (int32_t)((steps + p.chunk_steps - 1) / p.chunk_steps);
-      // second pass: pieces of the column tiles for as many, of 16 tiles at least
+      // pieces of the column tiles for eight workgroups a CU, of 16 tiles at least
       const int64_t keys = kWaves * (s.head_dim == 256 ? 32 : 64);
       const int64_t units = (int64_t)s.num_seqs * s.num_kv_heads * ((s.max_context + keys - 1) / keys);
       const int64_t columns = ((int64_t)s.max_q_len * group + 31) / 32;
@@ -118,11 +107,10 @@ Plan plan_call(const Shape& s) {
       p.column_tiles = (int32_t)((columns + pieces - 1) / pieces);
       p.column_pieces = (int32_t)((columns + p.column_tiles - 1) / p.column_tiles);
       const size_t tiles = ((size_t)s.num_q_tokens * group / 32 + s.num_seqs) * s.num_kv_heads;
-      p.chunk_bytes = align256(tiles * (32 * 8 * (size_t)(1 + p.chunk_pieces) +
-                                        (size_t)s.terms * s.head_dim * 64));
+      p.column_bytes = align256(tiles * (32 * 8 + (size_t)s.terms * s.head_dim * 64));
       if (p.column_pieces > 1)
-        p.chunk_bytes += align256((size_t)s.num_seqs * s.num_kv_heads * p.column_pieces *
-                                  p.score_stride * sizeof(float));
+        p.column_bytes += align256((size_t)s.num_seqs * s.num_kv_heads * p.column_pieces *
+                                   p.score_stride * sizeof(float));
     }
   }
   return p;
@@ -284,16 +272,17 @@ int bounded_attention(const Call& c) {
   chunk.pf_min_rows = only_chunks ? 1 : 2;
   chunk.max_context = c.max_context_len;
   chunk.pf_ws = static_cast<float*>(c.workspace);
-  chunk.pf_bytes = need;
+  chunk.pf_bytes = plan.prefill_bytes;
   chunk.sinks = c.sinks;
-  // (the build with sinks also rounds less for f16 and fp32 queries)
-  const int rc = c.sinks > 0 || c.q_dtype != ASTR_BF16 ? launch_prefill_sinks(chunk, c.q_dtype, s)
-                                                       : launch_prefill(chunk, c.q_dtype, s);
+  if (w != nullptr) a.column_ws = reinterpret_cast<float*>(ws + plan.prefill_bytes);
+  chunk.column_ws = a.column_ws;
+  // (the build with sinks also keeps what the key weights need, and rounds less for f16 and fp32
+  // queries)
+  const bool sinks_build = c.sinks > 0 || w != nullptr || c.q_dtype != ASTR_BF16;
+  const int rc = sinks_build ? launch_prefill_sinks(chunk, c.q_dtype, s)
+                             : launch_prefill(chunk, c.q_dtype, s);
   if (rc != 0 || w == nullptr) return rc;
-  a.chunk_ws = static_cast<float*>(c.workspace);
   a.min_rows = chunk.pf_min_rows;
-  a.chunk_pieces = plan.chunk_pieces;
-  a.chunk_steps = plan.chunk_steps;
   a.column_pieces = plan.column_pieces;
   a.column_tiles = plan.column_tiles;
   return launch_chunk_weights(a, c.q_dtype, s);

@@ -27,11 +27,10 @@ struct BoundedArgs : AttnArgs {
   // base-2 scores of every key, [num_seqs * num_kv_heads * group][score_stride]; weights only
   float* scores;
   int64_t score_stride;
-  // chunks (key weights, chunk_weights.hip): their workspace; the first pass's pieces of the keys
-  // and their steps of 64 keys; the second's pieces of the column tiles and their length
-  float* chunk_ws;
+  // chunks (key weights, chunk_weights.hip): their workspace; the pieces of the column tiles and
+  // their length
+  float* column_ws;
   int32_t min_rows;  // fewest queries of a row the chunk kernels take
-  int32_t chunk_pieces, chunk_steps;
   int32_t column_pieces, column_tiles;
 };
 
@@ -82,11 +81,43 @@ __device__ __forceinline__ int64_t weight_row(const BoundedArgs& a, int seq, boo
   return row;
 }
 
+// What the attention launch leaves of each query column (token, head of the group) of a chunk for
+// the sums over the columns (chunk_weights.hip): {factor, lse}, with score = factor * k_scale *
+// (codes . operand) in base 2 and an lse of +inf where the column adds no weight, and the f16
+// operands in MFMA order. In tiles of 32 columns: those of sequence s begin at q0 * G / 32 + s, of
+// `tiles` per KV head. Behind them the column pieces' sums, one row of score_stride keys per
+// (sequence, KV head) and piece.
+struct ColumnWs {
+  typedef float pair_t __attribute__((ext_vector_type(2)));
+  pair_t* cols;
+  half8_t* ops;
+  float* sums;
+  int64_t tiles;
+  int group;
+  __host__ __device__ ColumnWs(const AttnArgs& a, float* base, int op_halves) {
+    group = a.num_q_heads / a.cache.num_kv_heads;
+    tiles = (int64_t)a.num_q_tokens * group / 32 + a.num_seqs;
+    const int64_t columns = tiles * a.cache.num_kv_heads * 32;
+    cols = reinterpret_cast<pair_t*>(base);
+    ops = reinterpret_cast<half8_t*>(cols + columns);
+    sums = reinterpret_cast<float*>(ops + columns * (op_halves / 8));
+  }
+  // the first tile of (seq, kvh), whose queries begin at q0
+  __device__ int64_t tile0(int seq, int kvh, int q0) const {
+    return (int64_t)kvh * tiles + (int64_t)q0 * group / 32 + seq;
+  }
+};
+// A column's log2 of the sum over its keys; +inf where it saw none or its scores are not finite.
+__device__ __forceinline__ float column_lse(float m, float l) {
+  return l > 0.f ? m + __builtin_amdgcn_logf(l) : INFINITY;
+}
+
 template <int KF> int launch_bounded_kf(const BoundedArgs& a, int32_t q_dtype, hipStream_t stream);
 template <int KF> int launch_chunk_weights_kf(const BoundedArgs& a, int32_t q_dtype, hipStream_t stream);
-// the chunked-prefill kernels with sinks (prefill.hip)
+// the chunked-prefill kernels with sinks or key weights (prefill.hip)
 struct SinkChunkArgs : ChunkArgs {
   int32_t sinks;
+  float* column_ws;  // ColumnWs of a call with key weights, else null
 };
 template <int KF> int launch_prefill_sinks_kf(const SinkChunkArgs& a, int32_t q_dtype, hipStream_t stream);
 #define ASTR_DECLARE_BOUNDED(KF)                                                             \

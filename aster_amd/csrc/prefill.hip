@@ -27,7 +27,8 @@
 // sharing a sequence's K/V then share that XCD's L2.
 //
 // Built once more with -DASTR_PF_SINKS=1: the first `sinks` keys stay visible beside the
-// window. A unit's blocks of sinks below its window run first, as key steps of their own.
+// window, a unit's blocks of sinks below its window running first, as key steps of their own; and
+// a call with key weights gets each column's operands and lse (ColumnWs).
 #include <algorithm>
 #include <climits>
 #include <cstddef>
@@ -48,7 +49,7 @@ constexpr int KF = ASTR_KF;  // this translation unit's code format
 #define ASTR_PF_SINKS 0
 #endif
 constexpr bool kSinks = ASTR_PF_SINKS != 0;
-// The kernels' arguments. sinks_of is 0 without sinks, which leaves no code.
+// The kernels' arguments. sinks_of is 0 and column_ws_of null without sinks, which leaves no code.
 using PrefillArgs = std::conditional_t<kSinks, SinkChunkArgs, ChunkArgs>;
 
 // How the V scales enter. Else (bf16 queries, and every query without sinks) V operands are
@@ -64,6 +65,10 @@ constexpr int kNoUnit = -120, kUnitBias = 128;
 __host__ __device__ __forceinline__ int sinks_of(const ChunkArgs& a) {
   if constexpr (kSinks) return static_cast<const SinkChunkArgs&>(a).sinks;
   else return 0;
+}
+__device__ __forceinline__ float* column_ws_of(const ChunkArgs& a) {
+  if constexpr (kSinks) return static_cast<const SinkChunkArgs&>(a).column_ws;
+  else return nullptr;
 }
 
 constexpr int kXcds = 8;
@@ -763,6 +768,12 @@ __device__ __forceinline__ void prefill_half(const PrefillLds<D>& L, int buf, in
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int i0 = 8 * w + 2 * j;
+        if constexpr (kSinks) {  // (key weights take the exact sum)
+          const float p0 = __builtin_amdgcn_exp2f(s[t][i0]), p1 = __builtin_amdgcn_exp2f(s[t][i0 + 1]);
+          l[t] += p0 + p1;
+          pop[t][w][j] = pack2<_Float16>(p0, p1);
+          continue;
+        }
         const uint32_t pair = pack2<_Float16>(__builtin_amdgcn_exp2f(s[t][i0]),
                                               __builtin_amdgcn_exp2f(s[t][i0 + 1]));
         l[t] = __builtin_amdgcn_fdot2(__builtin_bit_cast(half2_t, pair),
@@ -843,6 +854,11 @@ __device__ __forceinline__ void acc_run(const float16v_t (&acc)[D / 32], int x, 
     for (int n = 0; n < D / 32; ++n) v[y * (D / 32) + n] = acc[n][4 * x + y] * scale;
 }
 
+struct NoQueries {
+  template <typename Op>
+  __device__ __forceinline__ void operator()(int, const Op&, float) const {}
+};
+
 // One unit of the chunked-prefill kernels: the key blocks [b_lo, b_hi) of kv head kvh
 // (physical id of block b: blocks[b], a window of the arena's ids) against the
 // workgroup's query columns (column_of(f), bounds_of(wave)), through the key steps
@@ -851,15 +867,15 @@ __device__ __forceinline__ void acc_run(const float16v_t (&acc)[D / 32], int x, 
 // prologue() runs (in uniform control flow) once the first block id is on its way,
 // before any column is read: it returns false (uniformly) to end the unit there, with
 // nothing stored. mark(k) is called at the unit's timeline marks 2-5 (the tile kernel's
-// trace builds).
+// trace builds). queries(group, op, back) takes the operands of each column group once.
 template <typename QT, int D, int KS, typename ColumnOf, typename BoundsOf, typename Store,
-          typename Prologue, typename Mark>
+          typename Prologue, typename Mark, typename Queries = NoQueries>
 __device__ __forceinline__ void prefill_unit(const AttnArgs& a, PrefillLds<D>& L, int kvh,
                                              int b_lo, int b_hi, const int32_t* blocks, int q0,
                                              int t0, ColumnOf column_of, BoundsOf bounds_of,
                                              Store store, Prologue prologue, Mark mark,
                                              SinkSpan sink = SinkSpan{0, 0, 0}, int step0 = 0,
-                                             int all_steps = 0) {
+                                             int all_steps = 0, Queries queries = Queries{}) {
   using Shape = PrefillShape<D, KS>;
   constexpr int NT = Shape::NT;
   constexpr int kRowsN = D / 32;
@@ -922,6 +938,7 @@ __device__ __forceinline__ void prefill_unit(const AttnArgs& a, PrefillLds<D>& L
   for (int t = 0; t < NT; ++t) {
     back[t] = query_operand<QT, D>(qraw[t], hi[t] >= 0, qop[t]);
     scaled |= __ballot(back[t] != 1.f) != 0;
+    if (half == 0) queries(group, qop[t], back[t]);
   }
   const WaveBounds wb = bounds_of(group);
   mark(2);
@@ -1094,6 +1111,39 @@ __device__ __forceinline__ void prefill_unit(const AttnArgs& a, PrefillLds<D>& L
     store(t, acc[t], m[t], sum32(l[t]), kExactV && KF == kE4M3 ? ve + 8 : ve, column_of(f));
   }
   mark(5);
+}
+
+// Key weights: what column group `group` of a tile leaves for the sums over the columns (see
+// ColumnWs), its queries once and the lse with the output. A column that is not finite enters as
+// zeros; its lse comes out infinite.
+template <typename QT, int D, int G>
+__device__ __forceinline__ void keep_query(const PrefillArgs& a, int seq, int kvh, int q0, int t0, int t1,
+                                           int group, const QOp<QT, D>& q, float back) {
+  if constexpr (kSinks) {
+    if (column_ws_of(a) == nullptr || t0 + group * 32 / G >= t1) return;
+    using Op = QOp<QT, D>;
+    const ColumnWs ws(a, column_ws_of(a), Op::kTerms * D);
+    const int64_t tile = ws.tile0(seq, kvh, q0) + t0 * G / 32 + group;
+    const int lane = lane_id();
+    const bool finite = __builtin_isfinite(back);
+#pragma unroll
+    for (int t = 0; t < Op::kTerms; ++t)
+#pragma unroll
+      for (int cc = 0; cc < D / 16; ++cc)
+        ws.ops[((tile * Op::kTerms + t) * (D / 16) + cc) * kWave + lane] =
+            finite ? q.op[t][cc] : half8_t{};
+    if (lane < 32)
+      ws.cols[tile * 32 + lane][0] = finite ? back * a.qk_scale_log2 * code_scale<KF>() : 0.f;
+  }
+}
+template <typename QT, int D, int G>
+__device__ __forceinline__ void keep_lse(const PrefillArgs& a, int seq, int kvh, int q0, int t0, int t1,
+                                         int group, float m, float l, int lane) {
+  if constexpr (kSinks) {
+    if (column_ws_of(a) == nullptr || t0 + group * 32 / G >= t1 || lane >= 32) return;
+    const ColumnWs ws(a, column_ws_of(a), QOp<QT, D>::kTerms * D);
+    ws.cols[(ws.tile0(seq, kvh, q0) + t0 * G / 32 + group) * 32 + lane][1] = column_lse(m, l);
+  }
 }
 
 // A unit of the prefill launch: query tile `tile` of sequence `seq`.
@@ -1283,11 +1333,15 @@ __global__ __launch_bounds__(256, (prefill_occupancy<QT, D>())) void prefill_mfm
     } else if (c.valid) {
       store_column<QT, D>(a, acc, up / fmaxf(l, FLT_MIN), q0 + c.tok, c.head, lane);
     }
+    if (part == nullptr) keep_lse<QT, D, G>(a, seq, kvh, q0, t0, t1, wave_id, m, c.valid ? l : 0.f, lane);
+  };
+  auto queries = [&](int group, const QOp<QT, D>& q, float back) __attribute__((always_inline)) {
+    if (piece == 0) keep_query<QT, D, G>(a, seq, kvh, q0, t0, t1, group, q, back);
   };
   prefill_unit<QT, D, KS>(a, L, kvh, span.b_lo, span.b_hi,
                       a.block_tables + (int64_t)seq * a.bt_stride, q0, t0, column_of,
                       bounds_of, store, []() { return true; }, [](int) {}, sink_span(a, span),
-                      step0, nsteps);
+                      step0, nsteps, queries);
 }
 
 constexpr int kMostPieces = 16;
@@ -1377,6 +1431,8 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillArgs a) {
   }
   const int f = group * 32 + (lane & 31);
   const int token = span.t0 + f / G;
+  if (part == 0)
+    keep_lse<QT, D, G>(a, u.seq, kvh, u.q0, span.t0, span.t1, group, mx, token < span.t1 ? l : 0.f, lane);
   if (token >= span.t1) return;
   const float inv = 1.f / fmaxf(l, FLT_MIN);
   float o[D / 8];
