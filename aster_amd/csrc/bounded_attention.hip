@@ -276,11 +276,7 @@ int bounded_attention(const Call& c) {
   chunk.sinks = c.sinks;
   if (w != nullptr) a.column_ws = reinterpret_cast<float*>(ws + plan.prefill_bytes);
   chunk.column_ws = a.column_ws;
-  // (the build with sinks also keeps what the key weights need, and rounds less for f16 and fp32
-  // queries)
-  const bool sinks_build = c.sinks > 0 || w != nullptr || c.q_dtype != ASTR_BF16;
-  const int rc = sinks_build ? launch_prefill_sinks(chunk, c.q_dtype, s)
-                             : launch_prefill(chunk, c.q_dtype, s);
+  const int rc = launch_prefill_sinks(chunk, c.q_dtype, s);
   if (rc != 0 || w == nullptr) return rc;
   a.min_rows = chunk.pf_min_rows;
   a.column_pieces = plan.column_pieces;

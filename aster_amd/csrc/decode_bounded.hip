@@ -15,9 +15,10 @@
 // cache, once lse is known; reading the keys again instead would double the call's bytes.
 //
 // Queries of 16 bits: int8 codes meet three int8 terms of the query (exact products, 22
-// bits of the query), FP8 codes an f16 query; softmax weights enter the output's products
-// rounded to f16, the sums in fp32 before that rounding. fp32 queries: FP8 codes meet two
-// f16 terms of the query, and the weights enter as two f16 terms (22 bits).
+// bits of the query), FP8 codes an f16 query (two f16 terms of an fp32 one); the softmax weights
+// enter the output's products rounded to f16 where the output is bf16, else as two f16 terms (22
+// bits; one term, 2^-12 beside an f16 output's own 2^-12, saved 3 % of a call: 48 rows of FP8 codes
+// 15.2 us, now 15.6). The sums are fp32, before that rounding.
 #include <climits>
 
 #include "bounded_common.h"
@@ -213,7 +214,7 @@ __device__ __forceinline__ float4_t bounded_block(const char* st,
     for (int n = 0; n < NPV; ++n) acc[n] *= alpha;
     m = mn;
   }
-  constexpr int kTerms = sizeof(QT) == 4 ? 2 : 1;
+  constexpr int kTerms = __is_same(QT, bf16_t) ? 1 : 2;
   half4_t pop[kTerms];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {

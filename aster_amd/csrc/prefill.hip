@@ -52,15 +52,17 @@ constexpr bool kSinks = ASTR_PF_SINKS != 0;
 // The kernels' arguments. sinks_of is 0 and column_ws_of null without sinks, which leaves no code.
 using PrefillArgs = std::conditional_t<kSinks, SinkChunkArgs, ChunkArgs>;
 
-// How the V scales enter. Else (bf16 queries, and every query without sinks) V operands are
-// rounded products of code and scale and softmax weights are rounded to f16: three roundings of
-// 2^-11 per term, far below a bf16 output's own 2^-9 but above an f16 output's. Here, for f16 and
-// fp32 queries, the V operands are the codes, exactly, and the scale enters with the weight in
-// fp32, ahead of one rounding to f16 (two f16 terms for fp32 queries): errors of f16 outputs
-// against 64 bits 4.0e-4 -> 2.9e-4 (2.1e-4 is their own rounding). The product enters in units
-// of 2^ve: the largest V scale so far in [2^4, 2^7) of it, as weights are up to 2^8.
-template <typename QT>
-constexpr bool exact_v() { return kSinks && !std::is_same<QT, bf16_t>::value; }
+// How the V scales enter. Without sinks V operands are rounded products of code and scale, of at
+// least f16's step 2^-24, and softmax weights, rounded to f16, have rounded sums: far below a bf16
+// output's own 2^-9 (of V values above 2^-15), but not an f16 output's. With them (and for key
+// weights, which need the exact sums) the V operands are the codes, exactly, and the scale enters
+// with the weight in fp32, ahead of one f16 term for bf16 queries and two for others: V values of
+// any magnitude, and errors of f16 outputs against 64 bits 4.0e-4 -> 2.1e-4, which is their own
+// rounding (one term: 2.9e-4). 512 tokens on 16000 with a window of 4096, bf16,
+// 64.2 us -> 68.8; ragged FP8
+// prompts of a head-dim 64 model, f16, 43.4 us a call with one term, 48.5 with two. The product
+// enters in units of 2^ve: the largest V scale so far in [2^4, 2^7) of it, as weights are up to 2^8.
+constexpr bool kExactV = kSinks;
 constexpr int kNoUnit = -120, kUnitBias = 128;
 __host__ __device__ __forceinline__ int sinks_of(const ChunkArgs& a) {
   if constexpr (kSinks) return static_cast<const SinkChunkArgs&>(a).sinks;
@@ -69,6 +71,18 @@ __host__ __device__ __forceinline__ int sinks_of(const ChunkArgs& a) {
 __device__ __forceinline__ float* column_ws_of(const ChunkArgs& a) {
   if constexpr (kSinks) return static_cast<const SinkChunkArgs&>(a).column_ws;
   else return nullptr;
+}
+
+// A row's length within its table and, with sinks or key weights, the host's bound.
+__device__ __forceinline__ int row_ctx(const ChunkArgs& a, int ctx, bool report) {
+  if constexpr (kSinks) {
+    const int cap = min((int)min((int64_t)a.bt_stride * kBlockTokens, (int64_t)INT_MAX), a.max_context);
+    if (ctx > cap) {
+      if (report) atomicOr(a.err_flag, ASTR_FLAG_BAD_INDEX);
+      return cap;
+    }
+  }
+  return clamp_ctx(a, ctx, report);
 }
 
 constexpr int kXcds = 8;
@@ -177,7 +191,7 @@ __device__ int plan_rows(const ChunkArgs& a, int tq, int* tab, int* s_wsum, int&
       n = seq_queries(a, s, q0);
       if (n >= a.pf_min_rows) {
         ctx_raw = a.context_lens[s];
-        const TileSpan sp = tile_span(a, clamp_ctx(a, ctx_raw, false), n, (n - 1) / tq, tq);
+        const TileSpan sp = tile_span(a, row_ctx(a, ctx_raw, false), n, (n - 1) / tq, tq);
         key = sp.b_hi - sp.b_lo;
         tiles = (n + tq - 1) / tq;
       }
@@ -463,7 +477,7 @@ __device__ __forceinline__ void load_raw(const AttnArgs& a, int id, int kvh, int
 // The wave's block into the operands of buffer `buf`, as block `w` of its step. The V
 // exponent e is the unit's current `ve`, or more where a scale exceeds `vlim` = 2^(15 + ve)
 // / format_max, so that every f16 product stays below 2^15.
-template <int D, bool kPad, bool kExactV>
+template <int D, bool kPad>
 __device__ __forceinline__ void convert_raw(const AttnArgs& a, const RawBlock<D>& b,
                                             PrefillLds<D>& L, int buf, int w, int lane, bool masks,
                                             int ve, float vlim) {
@@ -733,10 +747,10 @@ __device__ __forceinline__ void prefill_half(const PrefillLds<D>& L, int buf, in
       for (int j = 0; j < 16; ++j) s[t][j] -= shift;
     }
   }
-  // weights rounded to f16; the sums take the same rounded weights as the numerator
+  // weights rounded to f16; the sums take the same rounded weights as the numerator (kExactV:
+  // as they are)
   typedef uint32_t word4_t __attribute__((ext_vector_type(4)));
-  constexpr bool kExactV = exact_v<QT>();
-  constexpr int kPTerms = kExactV && sizeof(QT) == 4 ? 2 : 1;
+  constexpr int kPTerms = kExactV && !__is_same(QT, bf16_t) ? 2 : 1;
   word4_t pop[NT][2], pop2[kPTerms == 2 ? NT : 1][2];
   if constexpr (kExactV) {
     // times the V scales in the unit, then rounded; the sums take the weights as they are
@@ -768,12 +782,6 @@ __device__ __forceinline__ void prefill_half(const PrefillLds<D>& L, int buf, in
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int i0 = 8 * w + 2 * j;
-        if constexpr (kSinks) {  // (key weights take the exact sum)
-          const float p0 = __builtin_amdgcn_exp2f(s[t][i0]), p1 = __builtin_amdgcn_exp2f(s[t][i0 + 1]);
-          l[t] += p0 + p1;
-          pop[t][w][j] = pack2<_Float16>(p0, p1);
-          continue;
-        }
         const uint32_t pair = pack2<_Float16>(__builtin_amdgcn_exp2f(s[t][i0]),
                                               __builtin_amdgcn_exp2f(s[t][i0 + 1]));
         l[t] = __builtin_amdgcn_fdot2(__builtin_bit_cast(half2_t, pair),
@@ -956,8 +964,7 @@ __device__ __forceinline__ void prefill_unit(const AttnArgs& a, PrefillLds<D>& L
   }
   // The PV accumulators are in units of 2^-ve: ve is the largest block exponent so far
   // (0 unless a block's V scales need more, see convert_raw); vlim is its scale limit.
-  // exact_v: the unit, kNoUnit before the first block, and the largest scale it takes.
-  constexpr bool kExactV = exact_v<QT>();
+  // kExactV: the unit, kNoUnit before the first block, and the largest scale it takes.
   int ve = kExactV ? kNoUnit : 0;
   float vlim = kExactV ? -1.f : 32768.f / format_max<KF>();
   float vunit = 1.f;
@@ -970,7 +977,7 @@ __device__ __forceinline__ void prefill_unit(const AttnArgs& a, PrefillLds<D>& L
   const int inner_hi = wb.any && inner_end > 0 ? inner_end / kStepKeys : 0;
   if (nsteps > 0) {
     if constexpr (!QOp<QT, D>::kAhead) load_step(0);
-    convert_raw<D, QOp<QT, D>::kPad, exact_v<QT>()>(a, raw, L, 0, wave, lane, masks, ve, vlim);
+    convert_raw<D, QOp<QT, D>::kPad>(a, raw, L, 0, wave, lane, masks, ve, vlim);
     if (nsteps > 1) load_step(1);
     __syncthreads();
   }
@@ -1057,7 +1064,7 @@ __device__ __forceinline__ void prefill_unit(const AttnArgs& a, PrefillLds<D>& L
     }
     if (i + 1 < nsteps) {
       // the other buffer was last read in step i - 1, before the barrier that ended it
-      convert_raw<D, QOp<QT, D>::kPad, exact_v<QT>()>(a, raw, L, buf ^ 1, wave, lane, masks, ve, vlim);
+      convert_raw<D, QOp<QT, D>::kPad>(a, raw, L, buf ^ 1, wave, lane, masks, ve, vlim);
       if (i + 2 < nsteps) load_step(i + 2);
     }
     __syncthreads();
@@ -1268,7 +1275,7 @@ __global__ __launch_bounds__(256, (prefill_occupancy<QT, D>())) void prefill_mfm
   if (!unit_ref(a, TQ, tab, lds.wsum, lds.found, rows, head_unit % per_kv, u)) return;
   const int seq = u.seq, q0 = u.q0, n = u.n;
   const bool reporter = kvh == 0 && u.last && threadIdx.x == 0;
-  const int ctx = clamp_ctx(a, u.ctx_raw, reporter);
+  const int ctx = row_ctx(a, u.ctx_raw, reporter);
   // chunk longer than the context (a one-token row may be empty, as in a decode launch)
   if (ctx < n && n > 1 && reporter) atomicOr(a.err_flag, ASTR_FLAG_BAD_INDEX);
 
@@ -1403,7 +1410,7 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillArgs a) {
   const int kvh = unit / per_kv;
   UnitRef u;
   if (!unit_ref(a, TQ, tab, s_wsum, s_found, rows, unit % per_kv, u)) return;
-  const TileSpan span = tile_span(a, clamp_ctx(a, u.ctx_raw, false), u.n, u.tile, TQ);
+  const TileSpan span = tile_span(a, row_ctx(a, u.ctx_raw, false), u.n, u.tile, TQ);
   const int steps = tile_steps(a, span);
   const int pieces = min((steps + a.pf_steps - 1) / a.pf_steps, a.pf_pieces);
   if (pieces <= 1) return;

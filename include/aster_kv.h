@@ -468,8 +468,8 @@ int astr_paged_attention_i8_planned_append(
  *              bytes, 256-byte aligned (NULL allowed when that is 0); not shared by calls
  *              that overlap (two captured graphs replayed side by side need one each).
  * Only the blocks of a sink or window key are read: table entries between them may hold any
- * id. Rows of fp32 queries with one token come out within fp32 rounding; chunks multiply
- * softmax weights rounded to f16, as astr_paged_attention_varlen_i8.
+ * id. Softmax weights enter the products with V as two f16 terms (22 bits), for bf16 queries as
+ * one; their sums are fp32.
  */
 int astr_paged_attention_i8_sinks(
     const astr_paged_kv* cache, const void* query, int32_t q_dtype, int64_t q_token_stride,

@@ -328,6 +328,58 @@ def test_non_finite_scores_are_reported_and_add_nothing(device):
         assert (kw.values[1, 0, :, :60].sum() > 0).all()
 
 
+@pytest.mark.parametrize("v_scale,k_scale,q_scale", [(1e-30, 1.0, 1.0), (1e30, 1.0, 1.0),
+                                                     (1.0, 40.0, 1.0), (1.0, 1e-6, 3e5),
+                                                     (1.0, 1e6, 1e-6)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_chunk_magnitudes(device, dtype, v_scale, k_scale, q_scale):
+    counts, lens = [70, 5, 40], [90, 5, 400]
+    cache, tables, _ = make_arena(device, lens, kv_heads=2, dim=128, v_scale=v_scale, k_scale=k_scale)
+    q = queries(device, sum(counts), 8, 128, dtype, scale=q_scale)
+    out = run_sinks(cache, tables, lens, q, 64, 4, counts)
+    check_rows(cache, tables, lens, q, out, counts, window=64, sinks=4)
+    kw = gathered(cache, lens, [0, 1, 2], counts=counts)
+    before = kw.values[:, 0].clone()
+    out = run_weights(cache, tables, lens, q, kw, [0, 1, 2], counts)
+    check_rows(cache, tables, lens, q, out, counts, kw.values[:, 0], before, [0, 1, 2])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_non_finite_query_leaves_the_others_weights(device, dtype):
+    cache, tables, _ = make_arena(device, [90], kv_heads=2, dim=64)
+    q = queries(device, 40, 2, 64, dtype)
+    plain = q.clone()
+    plain[7] = 0
+    q[7] = float("nan")
+    kw = KeyWeights(cache, rows=1, capacity=96)
+    with pytest.raises(ValueError, match="overflow"):
+        run_weights(cache, tables, [90], q, kw, [0], [40])
+    _, _, unit, every = attend_row(cache, tables[0], 90, plain)
+    without = attend_row(cache, tables[0], 58, plain[7:8])[3]  # token 7 sees 58 keys
+    every[:, :58] -= without
+    check_weights(kw.values[0, 0, :, :90], every, unit, terms=40)
+
+
+def test_chunks_past_the_host_bound_are_cut_and_reported(device):
+    counts, lens = [30, 20], [50, 90]
+    cache, tables, _ = make_arena(device, lens, kv_heads=1, dim=64)
+    q = queries(device, sum(counts), 2, 64, torch.bfloat16)
+    starts = on(device, np.array([0, 30, 50], np.int32))
+    args = (0, q, on(device, tables), on(device, np.asarray(lens, np.int32)))
+    with pytest.raises(ValueError, match="outside the KV arena"):
+        cache.paged_attention(*args, max_context_len=60, window=16, sinks=2, query_start_loc=starts,
+                              max_query_len=30, check=True)
+    kw = KeyWeights(cache, rows=2, capacity=96)
+    kw.values.fill_(0.5)
+    before = kw.values[:, 0].clone()
+    out = torch.empty_like(q)
+    with pytest.raises(ValueError, match="outside the KV arena"):
+        cache.paged_attention_weights(*args, kw.select([0, 1]), max_context_len=60, out=out,
+                                      query_start_loc=starts, max_query_len=30, check=True)
+    # the row within the bound as ever, the other one as if it ended there
+    check_rows(cache, tables, [50, 60], q, out, counts, kw.values[:, 0], before, [0, 1])
+
+
 def test_lengths_and_ids_out_of_range_are_reported(device):
     lens = [50, 60]
     cache, tables, _ = make_arena(device, lens, kv_heads=1, dim=64)
