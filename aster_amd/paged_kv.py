@@ -69,6 +69,7 @@ class PagedKVCache:
         self.err_flag = torch.zeros(1, dtype=torch.int32, device=device)
         self._workspace = None
         self._bounded_sizes = {}  # workspace bytes by a call's sizes (a call to the library each)
+        self._stream_spaces = {}  # workspaces by stream
         self._descs = [self._make_desc(layer) for layer in range(num_layers)]
 
     # ---- descriptors --------------------------------------------------------
@@ -350,7 +351,8 @@ class PagedKVCache:
 
         ``sinks`` (with ``window``, causal, automatic split, no plan or packs): keys
         ``k < sinks`` stay visible beside the window. Only pages that hold a visible key
-        are read."""
+        are read. Captured into a graph, such a call takes a ``workspace`` of its own
+        (:meth:`bounded_workspace_bytes`), which replays that overlap must not share."""
         if sinks is not None:
             if type(sinks) is not int or sinks < 1 or window is None:
                 raise ValueError("sinks must be a positive int beside a window")
@@ -508,7 +510,9 @@ class PagedKVCache:
         :class:`~aster_amd.KeyWeights` (``KeyWeights.select``), one per sequence. The
         weights of the call's own tokens (the last ``n`` keys of a sequence with ``n``
         queries) start at 0, whatever the row held there; weights behind a sequence's length
-        are left as they are. A call that flags an error may have added its finite rows."""
+        are left as they are. A call that flags an error may have added its finite rows.
+        A call captured into a graph takes a ``workspace`` of its own
+        (:meth:`bounded_workspace_bytes`), which replays that overlap must not share."""
         num_seqs = block_tables.shape[0] if isinstance(block_tables, torch.Tensor) else 0
         require_rows(self, key_weights, num_seqs)
         if max_context_len > key_weights.weights.capacity:
@@ -540,6 +544,15 @@ class PagedKVCache:
         if self.device.index is None or self.device.index == torch.cuda.current_device():
             return contextlib.nullcontext()
         return torch.cuda.device(self.device)
+
+    def _stream_scratch(self, need, stream):
+        """The workspace of the calls on ``stream``, which follow one another there."""
+        with self._on_device():
+            if torch.cuda.is_current_stream_capturing():
+                raise ValueError("a captured call takes a workspace of its own")
+        if stream not in self._stream_spaces or self._stream_spaces[stream].numel() < need:
+            self._stream_spaces[stream] = torch.empty(need, dtype=torch.uint8, device=self.device)
+        return self._stream_spaces[stream]
 
     def _bounded_attention(self, layer, query, block_tables, context_lens, *, max_context_len,
                            scale=None, window=None, sinks=None, query_start_loc=None,
@@ -590,15 +603,15 @@ class PagedKVCache:
             num_seqs, num_q_heads, max_context_len, query.dtype, window=window, sinks=sinks,
             key_weights=key_weights is not None, num_query_tokens=num_tokens if packed else 0,
             max_query_len=max_query_len)
-        if need and workspace is None:
-            workspace = self._scratch(need)
-        elif need:
+        if need and workspace is not None:
             if (not isinstance(workspace, torch.Tensor) or workspace.dtype != torch.uint8
                     or workspace.device != self.device or not workspace.is_contiguous()):
                 raise ValueError("workspace must be a contiguous uint8 tensor on the cache device")
             if workspace.numel() < need:
                 raise ValueError(f"workspace of {need} bytes required")
         stream = torch.cuda.current_stream(self.device).cuda_stream
+        if need and workspace is None:
+            workspace = self._stream_scratch(need, stream)
         lib = _native.lib()
         args = [self._descs[layer], query.data_ptr(), _DTYPE_CODES[query.dtype], query.stride(0),
                 query.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
@@ -652,7 +665,8 @@ class PagedKVCache:
             raise ValueError("max_context_len exceeds the key weights' capacity")
         if dst_tables is not None:
             _check_index(dst_tables, "dst_tables", 2, self.device)
-            if dst_tables.shape[0] != num_seqs or                     dst_tables.shape[1] * self.block_size < min(keep, max_context_len):
+            if dst_tables.shape[0] != num_seqs or \
+                    dst_tables.shape[1] * self.block_size < min(keep, max_context_len):
                 raise ValueError("dst_tables must hold the tokens that stay, one row per sequence")
         if into is not None:
             weights.check(self, into, num_seqs, "into")

@@ -496,3 +496,40 @@ def test_positions_past_two_gigabytes(device):
     before = kw.values[:, 0].clone()
     out = run_weights(cache, high, [1000], chunk, kw, [0], [30])
     check_rows(cache, high, [1000], chunk, out, [30], kw.values[:, 0], before, [0])
+
+
+def test_streams_have_workspaces_of_their_own(device):
+    lens = [6000, 77]
+    cache, tables, _ = make_arena(device, lens, kv_heads=2, dim=128)
+    q = queries(device, 2, 8, 128, torch.bfloat16)
+    t, n = on(device, tables), on(device, np.asarray(lens, np.int32))
+    calls = [dict(max_context_len=6000, window=5000, sinks=9),  # in pieces
+             dict(max_context_len=6000, window=3500, sinks=3)]
+    want = [cache.paged_attention(0, q, t, n, **c) for c in calls]
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(20):
+        for side, call in zip(sides, calls):
+            with torch.cuda.stream(side):
+                got.append(cache.paged_attention(0, q, t, n, **call))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i % 2]) for i, o in enumerate(got))
+
+
+def test_a_captured_call_without_a_workspace_is_refused(device):
+    lens = [6000]
+    cache, tables, _ = make_arena(device, lens, kv_heads=2, dim=128)
+    q = queries(device, 1, 8, 128, torch.bfloat16)
+    t, n = on(device, tables), on(device, np.asarray(lens, np.int32))
+    assert cache.bounded_workspace_bytes(1, 8, 6000, q.dtype, window=5000, sinks=9) > 0
+    cell, graph = torch.zeros(4, device=device), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        cell.add_(1)
+        with pytest.raises(ValueError, match="workspace of its own"):
+            cache.paged_attention(0, q, t, n, max_context_len=6000, window=5000, sinks=9)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert (cell == 1).all()
+    cache.raise_errors()
