@@ -74,9 +74,7 @@ Plan plan_call(const Shape& s) {
   // every CU takes several units (128 rows, window 4096: 164 us a call against 167 with 8 waves and
   // 174 with 4), 8 where it takes one or none (48 rows, 4 KV heads, window 1024: 15.3 against
   // 17.8 and 20.2).
-  // Long rows of few units are cut into pieces in any case, which four waves balance better (16
-  // rows of 32768 keys with their weights, groups of 8: 291 us against 309 with 8).
-  p.waves = units > cus ? wide_waves(s.head_dim, s.weights && s.terms == 2) : units * blocks >= 256 * cus ? 4 : 8;
+  p.waves = units > cus ? wide_waves(s.head_dim, s.weights && s.terms == 2) : 8;
   // pieces: of 64 blocks a wave at most, and enough of them to give every CU 16 waves
   int64_t parts = (blocks + (int64_t)p.waves * kIdsPerWave - 1) / ((int64_t)p.waves * kIdsPerWave);
   const int64_t want = 16 * cus / (units * p.waves);

@@ -256,30 +256,47 @@ __device__ __forceinline__ float4_t bounded_block(const char* st,
   return float4_t{sc[0], sc[1], sc[2], sc[3]};
 }
 
-// Adds the weights of keys [t0, t1) of one (sequence, KV head): its scores (base 2) at
-// `scores` (one row per head, a.score_stride apart), lse (base 2) of its heads in `lse`. The
-// row's newest key starts at 0.
-__device__ __forceinline__ void add_weights(const BoundedArgs& a, const float* scores,
-                                            const float* lse, float* weights, int ctx, int t0,
-                                            int t1, int thread, int threads) {
-  const int G = a.group;
-  t1 = min(t1, min(ctx, a.kw.capacity));
-  for (int t = t0 + 4 * thread; t < t1; t += 4 * threads) {
-    float4_t sum = {0.f, 0.f, 0.f, 0.f};
-    for (int g = 0; g < G; ++g) {
-      const float4_t s = *reinterpret_cast<const float4_t*>(scores + g * a.score_stride + t);
-      const float e = lse[g];
-      if (e == INFINITY) continue;
+// The scores (base 2) of four keys from t on for up to eight heads from g0 on, on their way
+// together (one head at a time, the second launch of a row of 8192 keys took 6.3 us instead of 5.0).
+struct KeyScores {
+  static constexpr int kHeads = 8;
+  float4_t s[kHeads];
+  __device__ __forceinline__ void load(const BoundedArgs& a, const float* scores, int g0, int t) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sum[j] += __builtin_amdgcn_exp2f(s[j] - e);
-    }
-    if (t + 4 <= min(t1, ctx - 1)) {
-      *reinterpret_cast<float4_t*>(weights + t) += sum;
-    } else {
+    for (int i = 0; i < kHeads; ++i)
+      if (g0 + i < a.group)  // (uniform)
+        s[i] = *reinterpret_cast<const float4_t*>(scores + (g0 + i) * a.score_stride + t);
+  }
+  // Adds their weights; lse (base 2) of the group's heads, +inf where one adds none.
+  __device__ __forceinline__ void add(const BoundedArgs& a, const float* lse, int g0, float4_t& sum) const {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (t + j < t1) weights[t + j] = (t + j == ctx - 1 ? 0.f : weights[t + j]) + sum[j];
-    }
+    for (int i = 0; i < kHeads; ++i)
+      if (g0 + i < a.group) {
+        const float e = lse[g0 + i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[j] += e == INFINITY ? 0.f : __builtin_amdgcn_exp2f(s[i][j] - e);
+      }
+  }
+};
+
+// Adds the weights of keys t to t + 3, as far as they lie below t1, of one (sequence, KV head): its
+// scores at `scores` (one row per head, a.score_stride apart), those of the first heads in `first`.
+// The row's newest key starts at 0.
+__device__ __forceinline__ void add_keys(const BoundedArgs& a, const KeyScores& first, const float* scores,
+                                         const float* lse, float* weights, int ctx, int t, int t1) {
+  float4_t sum = {0.f, 0.f, 0.f, 0.f};
+  first.add(a, lse, 0, sum);
+  if (a.group > KeyScores::kHeads) {
+    KeyScores more;
+    more.load(a, scores, KeyScores::kHeads, t);
+    more.add(a, lse, KeyScores::kHeads, sum);
+  }
+  if (t + 4 <= min(t1, ctx - 1)) {
+    *reinterpret_cast<float4_t*>(weights + t) += sum;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (t + j < t1) weights[t + j] = (t + j == ctx - 1 ? 0.f : weights[t + j]) + sum[j];
   }
 }
 
@@ -408,7 +425,7 @@ __global__ __launch_bounds__(NW * kWave) void bounded_decode_kernel(BoundedArgs 
     // block i has landed once only the next one's loads may be on their way, and (WEIGHTS) the
     // score store issued after them: vector-memory operations complete in order (a padding load
     // among the younger ones makes this wait longer). Stores ahead of the next loads instead made
-    // every block wait for the one before's (16 rows of 32768 tokens, 64 heads: 269 us, now 266).
+    // every block wait for the one before's (16 rows of 32768 tokens, 64 heads: 1 % of the launch).
     if (i + 1 >= nblk) wait_vmcnt<0>();
     else if (WEIGHTS && i > 0) wait_vmcnt<S::kLoads + 1>();
     else wait_vmcnt<S::kLoads>();
@@ -491,10 +508,15 @@ __global__ __launch_bounds__(NW * kWave) void bounded_decode_kernel(BoundedArgs 
     if (reporter && v.ctx > a.kw.capacity) atomicOr(a.err_flag, ASTR_FLAG_BAD_INDEX);
     __threadfence_block();  // the scores, which other waves of the workgroup stored
     __syncthreads();
-    if (row >= 0)
-      add_weights(a, a.scores + unit * G * a.score_stride, lse,
-                  a.kw.values + row * a.kw.row_stride + kvh * a.kw.head_stride, v.ctx, 0, v.ctx,
-                  threadIdx.x, NW * kWave);
+    if (row < 0) return;
+    const float* const scores = a.scores + unit * G * a.score_stride;
+    float* const weights = a.kw.values + row * a.kw.row_stride + kvh * a.kw.head_stride;
+    const int t1 = min(v.ctx, a.kw.capacity);
+    for (int t = 4 * threadIdx.x; t < t1; t += 4 * NW * kWave) {
+      KeyScores first;
+      first.load(a, scores, 0, t);
+      add_keys(a, first, scores, lse, weights, v.ctx, t, t1);
+    }
   }
 }
 
@@ -513,6 +535,11 @@ __global__ __launch_bounds__(256) void bounded_merge_kernel(BoundedArgs a) {
   if (parts <= 1 || (tile > 0 && tile * kTileTokens >= v.ctx)) return;
   const int G = a.group;
   const int64_t head0 = (int64_t)seq * a.num_q_heads + kvh * G;
+  static_assert(kTileTokens == 4 * 256, "four keys a thread");
+  const int t = tile * kTileTokens + 4 * (int)threadIdx.x;
+  const float* const scores = WEIGHTS ? a.scores + head0 * a.score_stride : nullptr;
+  KeyScores first;  // on their way while lse is worked out
+  if (WEIGHTS && t < v.ctx) first.load(a, scores, 0, t);
   for (int g = wave; g < G; g += kWaves) {
     const float* ml = a.ws_ml + (head0 + g) * a.max_parts * 2;
     float M = -FLT_MAX;
@@ -545,10 +572,10 @@ __global__ __launch_bounds__(256) void bounded_merge_kernel(BoundedArgs a) {
     const bool reporter = tile == 0 && kvh == 0 && threadIdx.x == 0;
     const int64_t row = weight_row(a, seq, reporter);
     if (reporter && v.ctx > a.kw.capacity) atomicOr(a.err_flag, ASTR_FLAG_BAD_INDEX);
-    if (row >= 0)
-      add_weights(a, a.scores + ((int64_t)seq * a.cache.num_kv_heads + kvh) * G * a.score_stride,
-                  lse, a.kw.values + row * a.kw.row_stride + kvh * a.kw.head_stride, v.ctx,
-                  tile * kTileTokens, (tile + 1) * kTileTokens, threadIdx.x, 256);
+    const int t1 = min(v.ctx, a.kw.capacity);
+    if (row >= 0 && t < t1)
+      add_keys(a, first, scores, lse, a.kw.values + row * a.kw.row_stride + kvh * a.kw.head_stride, v.ctx,
+               t, t1);
   }
 }
 
