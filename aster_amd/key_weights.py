@@ -55,7 +55,9 @@ class KeyWeights:
     """Gathered weights ``values`` fp32 ``[rows, num_layers, num_kv_heads, capacity]`` of a
     :class:`PagedKVCache`'s keys, all zero at first. ``capacity``: the most tokens a sequence
     may have (rounded up to whole pages). A row may go to another sequence without being
-    cleared: a call sets the weights of its own new tokens and adds to those before them."""
+    cleared: a call sets the weights of its own new tokens and adds to those before them. So a
+    fork's row begins as a copy of its parent's values, and rows do not travel with archived
+    sequences."""
 
     def __init__(self, cache, *, rows, capacity):
         if any(type(v) is not int or v < 1 for v in (rows, capacity)):

@@ -196,7 +196,7 @@ class PagedStateArchive:
         """Fresh pages holding the archived tokens, as a new sequence of ``identity``;
         the snapshot stays archived until ``release``."""
         snapshot = self._catalog.lookup(handle, identity)
-        past = {"evicted": snapshot.evicted, "floor": snapshot.floor} if snapshot.floor else {}
+        past = {"evicted": snapshot.evicted, "floor": snapshot.floor} if snapshot.evicted else {}
         sequence = self.pool.restore_pages((snapshot.codes, snapshot.scales, snapshot.valid),
                                            identity=identity, length=snapshot.length,
                                            stream=self._copy_stream(), **past)

@@ -309,6 +309,10 @@ class PagedStatePool:
             check_budget(keep, recent, sinks)
             todo = [i for i, s in enumerate(sequences)
                     if s.length > keep or (cache.has_padding and s.length)]
+            # all that can be refused is refused before the first tokens and weights move
+            if any(sequences[i].length > weights.capacity for i in todo):
+                raise ValueError("a sequence exceeds the key weights' capacity")
+            cache.raise_errors()
             shared = [i for i in todo if any(self._page(ref).owners > 1 or self._page(ref).readers
                                              for ref in sequences[i].pages)]
             own = [i for i in todo if i not in set(shared)]
@@ -342,8 +346,9 @@ class PagedStatePool:
                 for index, ref in enumerate(pages[:count]):
                     page = self._page(ref)
                     page.valid = max(page.valid, min(self.block_size, length - index * self.block_size))
-                s.evicted += s.length - length
-                s.pages, s.length, s.floor = list(pages[:count]), length, length
+                if length < s.length:
+                    s.evicted, s.floor = s.evicted + s.length - length, length
+                s.pages, s.length = list(pages[:count]), length
             return tuple(s.length for s in sequences)
 
     def _table(self, rows):

@@ -334,6 +334,59 @@ def test_pool_eviction_refusals_change_nothing():
     pool.release(child)
 
 
+def test_pool_evictions_are_refused_before_anything_moves():
+    """A shared sequence is evicted ahead of the others: neither an error flagged earlier nor
+    another sequence's refusal may leave its weights moved."""
+    pool, kw, (a, b) = make(blocks=16, lens=(70, 60))
+    pool.fork(a)
+    weights, state = kw.values.clone(), [pool.materialize(s) for s in (a, b)]
+    short = KeyWeights(pool.cache, rows=2, capacity=64)
+    small = short.values.clone()
+    with pytest.raises(ValueError, match="capacity"):
+        pool.evict([b, a], short.select([0, 1]), keep=16)
+    pool.fork(b)
+    with pytest.raises(ValueError, match="capacity"):
+        pool.evict([b, a], short.select([0, 1]), keep=16)
+
+    def flagged():
+        raise ValueError("Quantized KV requires finite floating input")
+
+    real, pool.cache.raise_errors = pool.cache.raise_errors, flagged
+    with pytest.raises(ValueError, match="finite"):
+        pool.evict([a, b], kw.select([0, 1]), keep=16)
+    pool.cache.raise_errors = real
+    assert not pool.cache.calls and torch.equal(kw.values, weights) and torch.equal(short.values, small)
+    for s, before in zip((a, b), state):
+        assert s.evicted == s.floor == 0
+        assert all(torch.equal(x, y) for p, q in zip(pool.materialize(s), before) for x, y in zip(p, q))
+
+
+def test_an_eviction_that_drops_nothing_leaves_no_floor():
+    pool, kw, (a, b) = make(blocks=16, lens=(30, 20), padding=5)
+    c = pool.create("tenant")
+    ones = [(torch.ones((25, 2, 8)), torch.ones((25, 2, 8)))] * 2 + [(torch.ones(25, dtype=torch.bool),)]
+    pool.append_delta(c, ones)
+    assert pool.evict([c], kw.select([2]), keep=64) == (25,)
+    assert (c.evicted, c.floor) == (0, 0)
+    pool.truncate(c, 3)
+
+
+def test_archived_evictions_of_every_token_come_back():
+    """All tokens were padding and left; what came after is archived with their count."""
+    pool, kw, (seq,) = make(blocks=8, lens=(20,), padding=1)
+    assert pool.evict([seq], kw.select([0]), keep=8) == (0,)
+    assert (seq.evicted, seq.floor) == (20, 0)
+    pool.append_delta(seq, [(torch.ones((3, 2, 8)), torch.ones((3, 2, 8)))] * 2 +
+                      [(torch.ones(3, dtype=torch.bool),)])
+    archive = PagedStateArchive(pool)
+    archive._to_host = lambda s: (torch.zeros(1), torch.zeros(1), torch.zeros(1))
+    archive._copy_stream = lambda: None
+    got = {}
+    pool.restore_pages = lambda payloads, **kw: got.update(kw)
+    archive.restore(archive.put(seq), identity="tenant")
+    assert (got["evicted"], got["floor"]) == (20, 0)
+
+
 def test_archived_evictions_come_back():
     class Pool(PagedStatePool):
         def restore_pages(self, payloads, *, identity, length, stream=None, evicted=0, floor=0):
