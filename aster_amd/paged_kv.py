@@ -40,6 +40,8 @@ from .kv_quantization import KVQuantization, QuantizedKV, _DTYPE_CODES, require_
 
 DEFAULT_PARTITION_TOKENS = 0  # automatic: stream-K for bf16/fp16, else 512-token partitions
 
+_HERE = contextlib.nullcontext()
+
 
 class PagedKVCache:
     """Caller-owned device arena for ``num_layers`` layers of paged K/V in one of the
@@ -541,8 +543,8 @@ class PagedKVCache:
     def _on_device(self):
         """Makes the arena's device current for a call to the library, which plans for and
         launches on the current one."""
-        if self.device.index is None or self.device.index == torch.cuda.current_device():
-            return contextlib.nullcontext()
+        if self.device.index is None or self.device.index == torch._C._cuda_getDevice():
+            return _HERE
         return torch.cuda.device(self.device)
 
     def _raw_stream(self):
