@@ -533,3 +533,19 @@ def test_a_captured_call_without_a_workspace_is_refused(device):
     torch.cuda.synchronize()
     assert (cell == 1).all()
     cache.raise_errors()
+
+
+@pytest.mark.parametrize("counts", [[40, 1, 9], [20, 20, 20], [1, 1, 2]])
+def test_rows_behind_the_last_sequence_stay(device, counts):
+    lens = [300, 70, 20]
+    cache, tables, _ = make_arena(device, lens, kv_heads=2, dim=128)
+    q = queries(device, sum(counts) + 5, 8, 128, torch.bfloat16)
+    out = torch.full_like(q, 3.0)
+    run_sinks(cache, tables, lens, q, 50, 6, counts, out=out)
+    check_rows(cache, tables, lens, q, out, counts, window=50, sinks=6)
+    assert (out[sum(counts):] == 3).all()
+    kw = gathered(cache, lens, [2, 0, 1], counts=counts)
+    before = kw.values[:, 0].clone()
+    run_weights(cache, tables, lens, q, kw, [2, 0, 1], counts, out=out.fill_(3))
+    check_rows(cache, tables, lens, q, out, counts, kw.values[:, 0], before, [2, 0, 1])
+    assert (out[sum(counts):] == 3).all()

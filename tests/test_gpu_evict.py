@@ -186,3 +186,45 @@ def test_eviction_replays_in_a_graph(device):
             assert torch.equal(cache.scales.cpu()[page, :, :, :, slot], after[1][page, :, :, :, slot])
             assert torch.equal(kw.values[3 + r, :, :, :length].cpu(), after[2][3 + r, :, :, :length])
     cache.raise_errors()
+
+
+@pytest.mark.parametrize("apart", [False, True])
+def test_pages_past_two_gigabytes(device, apart):
+    """Codes that lie past 2^31 bytes of the arena, in place and into pages before them."""
+    from aster_amd import PagedKVCache
+
+    blocks = (1 << 31) // (2 * 8 * 16 * 128) + 70  # a block of one layer: 32 KB
+    cache = PagedKVCache(num_blocks=blocks, num_layers=1, num_kv_heads=8, head_dim=128, device=device)
+    gen = torch.Generator(device=device).manual_seed(3)
+    cache.codes[-64:] = torch.randint(-127, 128, cache.codes[-64:].shape, generator=gen, device=device,
+                                      dtype=torch.int8)
+    cache.scales[-64:] = torch.rand(cache.scales[-64:].shape, generator=gen, device=device)
+    kw = KeyWeights(cache, rows=1, capacity=1000)
+    kw.values.copy_(torch.rand(kw.values.shape, generator=gen, device=device))
+    high = np.arange(blocks - 64, blocks, dtype=np.int32)[None]
+    low = np.arange(3, 11, dtype=np.int32)[None] if apart else high
+    weights = kw.values[0, 0].cpu().numpy()
+    codes, scales = cache.codes[-64:].clone(), cache.scales[-64:].clone()
+    extra = {"dst_tables": on(device, low)} if apart else {}
+    got = evict(cache, kw, high, [1000], [0], keep=100, recent=10, sinks=2, **extra)
+    assert got.lengths.tolist() == [100]
+    at = torch.arange(100, device=device)
+    dst = torch.from_numpy(low[0].astype(np.int64)).to(device)[at // 16]
+    for h in range(8):
+        stay = chosen(weights[h, :1000], np.ones(1000, bool), 100, 2, 10)
+        src = torch.from_numpy(stay).to(device)
+        assert torch.equal(cache.codes[dst, 0, :, h, at % 16], codes[src // 16, 0, :, h, src % 16])
+        assert torch.equal(cache.scales[dst, 0, :, h, at % 16], scales[src // 16, 0, :, h, src % 16])
+
+
+def test_evictions_on_another_stream(device):
+    lens = [300, 90]
+    cache, tables, _, kw = setup(device, lens, padding=0.2)
+    before = state(cache, kw)
+    t, n, rows = on(device, tables), on(device, np.asarray(lens, np.int32)), kw.select([0, 1])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = cache.evict(t, n, rows, keep=64, recent=8, sinks=1, max_context_len=300)
+    side.synchronize()
+    check(cache, kw, tables, lens, [0, 1], before, got, keep=64, recent=8, sinks=1)
