@@ -88,13 +88,11 @@ def attend_row(cache, table, ctx, q, *, scale=None, window=None, sinks=0, layer=
 def check_out(got, want, absolute, unit, *, chunk=False):
     """``got`` within its rounding to the query's type (half a step), the roundings of the
     softmax weights and a score's error: every score is within ``unit`` 2^-21 (22 bits of the
-    query, fp32 sums), which moves a weight by e^(2 unit 2^-21) at most. Rows of one token: one
-    f16 rounding per weight (2^-11), or two f16 terms of fp32 queries (2^-22, and sums 2^-20).
-    Chunks of bf16 queries: the weights in numerator and sum, the V scale and its product, 2^-11
-    each; of others as rows of one token."""
+    query, fp32 sums), which moves a weight by e^(2 unit 2^-21) at most. bf16 queries: one f16
+    rounding per weight (2^-11), others two f16 terms (2^-22); sums and the rest 2^-20. Rows of
+    one token and chunks (``chunk``) alike."""
     eps = torch.finfo(got.dtype).eps / 2
-    rough = chunk and got.dtype == torch.bfloat16
-    term = 2 ** -9 if rough else (2 ** -20 if got.dtype == torch.float32 else 2 ** -11 + 2 ** -20)
+    term = 2 ** -20 + (2 ** -11 if got.dtype == torch.bfloat16 else 0)
     error = absolute * (term + 3 * unit * 2 ** -21)
     # (below 2^-24 of the largest V scale's unit an f16 weight is a subnormal: 2^-25 absolute)
     error = error + absolute.amax() * 2 ** -20 * (1 if got.dtype != torch.float32 else 2 ** -4)
